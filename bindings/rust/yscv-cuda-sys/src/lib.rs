@@ -88,6 +88,41 @@ pub struct yscv_cuda_decode_options {
     pub batch: c_int,
 }
 
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct yscv_cuda_rope {
+    pub theta: f64,
+    pub rotary_dim: usize,
+    pub interleaved: c_int,
+    pub scaling: c_int,
+    pub factor: f64,
+    pub original_positions: f64,
+    pub beta_fast: f64,
+    pub beta_slow: f64,
+    pub low_band: f64,
+    pub high_band: f64,
+    pub attention_factor: f64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct yscv_cuda_kv_pool {
+    pub d_k: *mut i8,
+    pub d_v: *mut i8,
+    pub d_kscale: *mut f32,
+    pub d_vscale: *mut f32,
+    pub layers: usize,
+    pub n_pages: usize,
+    pub n_kv: usize,
+    pub d_head: usize,
+    pub page: usize,
+    pub d_refs: *mut i32,
+    pub d_table: *mut i32,
+    pub d_length: *mut i32,
+    pub n_seq: usize,
+    pub max_pages: usize,
+}
+
 pub const YSCV_CUDA_OK: c_int = 0;
 pub const YSCV_CUDA_ERR_BAD_ARG: c_int = -1;
 pub const YSCV_CUDA_ERR_CUDA: c_int = -2;
@@ -97,6 +132,10 @@ pub const YSCV_CUDA_ERR_NO_DEVICE: c_int = -5;
 pub const YSCV_CUDA_WEIGHT_MATMUL_KN: c_int = 0;
 pub const YSCV_CUDA_WEIGHT_GEMM_NK: c_int = 1;
 pub const YSCV_CUDA_WEIGHT_GEMM_KN: c_int = 2;
+pub const YSCV_CUDA_ROPE_NONE: c_int = 0;
+pub const YSCV_CUDA_ROPE_LINEAR: c_int = 1;
+pub const YSCV_CUDA_ROPE_BANDED: c_int = 2;
+pub const YSCV_CUDA_ROPE_YARN: c_int = 3;
 pub const YSCV_CUDA_TP_HANDLE_BYTES: usize = 64;
 
 extern "C" {
@@ -197,4 +236,15 @@ extern "C" {
     pub fn yscv_cuda_decode_plan_free(plan: *mut yscv_cuda_decode_plan);
     pub fn yscv_cuda_decoder_layers_workspace(ctx: *mut yscv_cuda_ctx, layers: *const yscv_cuda_decode_layer, n_layers: usize, hidden: usize, inter: usize, n_q: usize, n_kv: usize, d_head: usize, batch: usize, seq: usize, bytes: *mut usize) -> c_int;
     pub fn yscv_cuda_decoder_layers_dev(ctx: *mut yscv_cuda_ctx, layers: *const yscv_cuda_decode_layer, n_layers: usize, hidden: usize, inter: usize, n_q: usize, n_kv: usize, d_head: usize, max_seq: usize, eps: f32, rope_theta: f32, kv_int8: c_int, batch: usize, seq: usize, d_pos: *const i32, d_x: *mut f32, d_final_gamma: *const f32, d_last: *mut f32, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn yscv_cuda_rope_dev(ctx: *mut yscv_cuda_ctx, d_x: *const f32, x_stride: usize, rows: usize, n_heads: usize, d_head: usize, d_pos: *const i32, rope: *const yscv_cuda_rope, d_out: *mut f32, out_stride: usize) -> c_int;
+    pub fn yscv_cuda_kv_block_append_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_k: *const f32, d_v: *const f32, row_stride: usize, d_offsets: *const i32, d_start: *const i32, most_rows: usize) -> c_int;
+    pub fn yscv_cuda_kv_block_read_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_offsets: *const i32, d_start: *const i32, most_rows: usize, d_k_out: *mut f32, d_v_out: *mut f32, row_stride: usize) -> c_int;
+    pub fn yscv_cuda_kv_block_attention_workspace(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, n_q: usize, rows: usize, most_rows: usize, bytes: *mut usize) -> c_int;
+    pub fn yscv_cuda_kv_block_attention_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_q: *const f32, q_stride: usize, n_q: usize, d_offsets: *const i32, d_start: *const i32, rows: usize, most_rows: usize, causal: c_int, window: usize, scale: f32, d_out: *mut f32, out_stride: usize, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn yscv_cuda_kv_pages_workspace(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, bytes: *mut usize) -> c_int;
+    pub fn yscv_cuda_kv_pages_extend_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, d_offsets: *const i32, rows: usize, d_start: *mut i32, d_pos: *mut i32, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn yscv_cuda_kv_pages_trim_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, d_seqs: *const i32, d_keep: *const i32, count: usize) -> c_int;
+    pub fn yscv_cuda_kv_pages_fork_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, d_src: *const i32, d_dst: *const i32, count: usize) -> c_int;
+    pub fn yscv_cuda_kv_pages_compact_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn yscv_cuda_kv_pages_copy_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, d_src: *const i32, d_dst: *const i32, count: usize) -> c_int;
 }

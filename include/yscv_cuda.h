@@ -80,7 +80,8 @@ void yscv_cuda_ctx_destroy(yscv_cuda_ctx *ctx);
 int yscv_cuda_ctx_synchronize(yscv_cuda_ctx *ctx);
 /* Reads and clears the device-side status word (0 = none): 1 a bounded wait on a copy
  * barrier ran out, 2 a bounded wait on another CTA or another GPU ran out, 3 a sequence
- * position outside [0, max_seq) was given to a cache append (nothing was appended). */
+ * position outside [0, max_seq) was given to a cache append (nothing was appended), 4 a page or sequence number that
+ * a call on a paged cache cannot use, 5 no free page left in a pool. */
 int yscv_cuda_ctx_device_status(yscv_cuda_ctx *ctx, int *status);
 const char *yscv_cuda_last_error(void);
 /* Counterpart of runtime_dispatch_report() (crates/yscv-kernels/src/core.rs:30-137):
@@ -659,6 +660,136 @@ int yscv_cuda_decoder_layers_dev(yscv_cuda_ctx *ctx, const yscv_cuda_decode_laye
                                  float rope_theta, int kv_int8, size_t batch, size_t seq,
                                  const int32_t *d_pos, float *d_x, const float *d_final_gamma,
                                  float *d_last, void *d_workspace, size_t workspace_bytes);
+
+/* ---- sequences of different lengths: rotary positions and a paged 8-bit cache ---------------
+ * No counterpart in the reference, whose decoding runs one sequence, or several at one position
+ * (apps/llm-bench/src/main.rs:491-561), over contiguous caches (crates/yscv-onnx/src/runner/kv_cache.rs).
+ * The rows of a call are ragged: sequence i of a pool has rows d_offsets[i] .. d_offsets[i + 1] - 1
+ * (d_offsets [n_seq + 1], rising, d_offsets[0] = 0) at positions d_start[i], d_start[i] + 1, ...;
+ * d_start[i] < 0 says that it takes no part. Rows of sequences that take no part and rows behind
+ * the last one are left as they were. `most_rows` is the largest number of rows of a sequence that
+ * the caller expects: it sizes grids and chooses kernels, a sequence with more of them is served all
+ * the same. All of it lies in device memory, so that a step can be captured and replayed while the
+ * sequences grow. Status words: 3 a position that the page table has no room for, 4 a page or
+ * sequence number that the call cannot use (what it stands for is left out), 5 no free page. */
+
+/* Rotary positions of the first n_heads heads of rows x_stride floats apart (the q and k heads of
+ * fused [q | k | v] rows), row r at position d_pos[r]; a negative position leaves the row of d_out as it
+ * was. d_out == d_x (and equal strides) turns in place, other overlaps are not allowed. Pairs are
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`; values past rotary_dim pass through.
+ * Pair i turns by position * w_i, w_i = theta^(-2 i / rotary_dim), stretched for long contexts:
+ *   LINEAR  w_i / factor
+ *   BANDED  by the turns of a pair over original_positions: at most low_band w_i / factor, at least
+ *           high_band w_i, blended between
+ *   YARN    the same with a ramp over the pairs, from the one that makes beta_fast turns over
+ *           original_positions to the one that makes beta_slow
+ * attention_factor multiplies cosine and sine (0: 0.1 ln(factor) + 1 with YARN, else 1). Angles are
+ * formed in fp64. rotary_dim is even, at most d_head and 512. */
+enum {
+    YSCV_CUDA_ROPE_NONE = 0,
+    YSCV_CUDA_ROPE_LINEAR = 1,
+    YSCV_CUDA_ROPE_BANDED = 2,
+    YSCV_CUDA_ROPE_YARN = 3
+};
+typedef struct yscv_cuda_rope {
+    double theta;
+    size_t rotary_dim;
+    int interleaved;
+    int scaling;
+    double factor;
+    double original_positions;
+    double beta_fast, beta_slow;
+    double low_band, high_band;
+    double attention_factor;
+} yscv_cuda_rope;
+int yscv_cuda_rope_dev(yscv_cuda_ctx *ctx, const float *d_x, size_t x_stride, size_t rows, size_t n_heads,
+                       size_t d_head, const int32_t *d_pos, const yscv_cuda_rope *rope, float *d_out,
+                       size_t out_stride);
+
+/* A paged KV cache. A page is a block of `page` (16, 32, 64 or 128) consecutive tokens of one
+ * sequence, int8 with one f32 scale per page and KV head, keys and values apart. Tokens lie in
+ * groups of 16:
+ *   d_k       [layers][n_pages][n_kv][page / 16][d_head / 16][16 tokens][16]
+ *   d_v       [layers][n_pages][n_kv][page / 16][d_head][16 tokens]
+ *   d_kscale, d_vscale  [layers][n_pages][n_kv]
+ *   d_refs    [n_pages]: sequences that hold the page, 0 free
+ *   d_table   [n_seq][max_pages]: page numbers of a sequence in order, -1 where it has none
+ *   d_length  [n_seq]: its tokens
+ * The caller allocates everything (d_k, d_v 16-byte aligned) and starts with d_refs and d_length
+ * zero and d_table -1; a page's bytes and scales need no clearing. The pool of a call is described by
+ * value: the struct may change between calls, a captured graph keeps what it was captured with. */
+typedef struct yscv_cuda_kv_pool {
+    int8_t *d_k;
+    int8_t *d_v;
+    float *d_kscale;
+    float *d_vscale;
+    size_t layers, n_pages, n_kv, d_head, page;
+    int32_t *d_refs;
+    int32_t *d_table;
+    int32_t *d_length;
+    size_t n_seq, max_pages;
+} yscv_cuda_kv_pool;
+
+/* Writes keys and values (rows of n_kv * d_head floats, row_stride floats apart) into the pages of one
+ * layer at their positions. The scale of a block is fp32(m / 127), m its largest magnitude, at least 2^-100; a
+ * value is held as the whole number nearest to its quotient by the scale (exactly: ties to the even one).
+ * A page that already holds tokens in front of the new ones keeps its scale, or takes the larger one of
+ * the new tokens and rounds what it holds once more. A NaN is held as 0, an infinity as +-127; neither
+ * counts for the scale. Pages that sequences share have to be made their own first
+ * (yscv_cuda_kv_pages_extend_dev does). d_head is a multiple of 16, at most 256. */
+int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_k,
+                                  const float *d_v, size_t row_stride, const int32_t *d_offsets,
+                                  const int32_t *d_start, size_t most_rows);
+/* The cached rows at the positions of a ragged call as f32, number times scale: the inverse. A row
+ * that has no page is left as it was. */
+int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer,
+                                const int32_t *d_offsets, const int32_t *d_start, size_t most_rows, float *d_k_out,
+                                float *d_v_out, size_t row_stride);
+
+/* Attention of the new rows over the pages of one layer: row s of sequence i (q_stride floats apart, n_q
+ * heads of d_head, n_q a multiple of n_kv) over the keys 0 .. d_start[i] + s, or all up to the sequence's last new
+ * row without `causal`; with window > 0 only over keys after its own position minus window. scale 0
+ * stands for 1 / sqrt(d_head). out rows are out_stride floats apart; a row that sees no key is 0.
+ * Products are exact in integers: queries and softmax weights enter as three 8-bit digits, cached
+ * values as they are. `rows` is the room in d_q and d_out, at least d_offsets[n_seq]. Rows with a NaN or an
+ * infinity in the query are NaN, and only those. d_head 64, 128 or 256. _workspace says how many
+ * bytes of device memory a call needs; calls that may overlap need one each. */
+int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows,
+                                           size_t most_rows, size_t *bytes);
+int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_q,
+                                     size_t q_stride, size_t n_q, const int32_t *d_offsets, const int32_t *d_start,
+                                     size_t rows, size_t most_rows, int causal, size_t window, float scale,
+                                     float *d_out, size_t out_stride, void *d_workspace, size_t workspace_bytes);
+
+/* Pages of a pool, all layers at once. Each call enqueues what it takes for the whole list; what it
+ * decides depends on the pool alone, not on timing.
+ * extend: sequence i gets room for d_offsets[i + 1] - d_offsets[i] more tokens: the lowest-numbered free
+ *   pages in the order of the sequences. A last page that is not full and that others share is
+ *   copied to a page of its own first (by every one of them that grows: the page itself is freed when
+ *   none is left). d_length grows; d_start receives the old length and d_pos [rows] the position of every
+ *   row, as the calls above take them. A sequence with no rows, one whose table is too short (status 3), and from
+ *   the first sequence that finds no page on all that need one (status 5) stay as they are, with -1 in
+ *   d_start and d_pos; so do rows behind the last one.
+ * trim: sequence d_seqs[j] keeps its first d_keep[j] tokens (d_keep null: none); pages that nobody holds
+ *   any more are free.
+ * fork: the empty sequence d_dst[j] shares all pages of d_src[j]. A source that is a destination of the same
+ *   call, a destination that is not empty or appears a second time: left out, status 4.
+ * compact: the used pages move to the lowest numbers, the k-th used one above into the k-th gap.
+ * copy: page d_dst[j] becomes what d_src[j] is; negative numbers are passed over. No page may be both a
+ *   source and a destination.
+ * _workspace: bytes that extend and compact need. */
+int yscv_cuda_kv_pages_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t *bytes);
+int yscv_cuda_kv_pages_extend_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_offsets,
+                                  size_t rows, int32_t *d_start, int32_t *d_pos, void *d_workspace,
+                                  size_t workspace_bytes);
+int yscv_cuda_kv_pages_trim_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_seqs,
+                                const int32_t *d_keep, size_t count);
+int yscv_cuda_kv_pages_fork_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_src,
+                                const int32_t *d_dst, size_t count);
+int yscv_cuda_kv_pages_compact_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, void *d_workspace,
+                                   size_t workspace_bytes);
+int yscv_cuda_kv_pages_copy_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_src,
+                                const int32_t *d_dst, size_t count);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,8 @@ from .lib import (  # noqa: F401
     Int4Weight,
     YscvCudaError,
     DecodePlan,
+    KvPool,
+    Rope,
     Registry,
     TpComm,
     int4_container_read,

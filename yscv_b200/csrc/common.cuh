@@ -109,6 +109,8 @@ enum : int {
     YSCV_DEV_MBARRIER_TIMEOUT = 1,
     YSCV_DEV_FLAG_TIMEOUT = 2,
     YSCV_DEV_POS_OVERFLOW = 3,  // the sequence position is outside [0, max_seq): nothing was appended
+    YSCV_DEV_BAD_NUMBER = 4,    // paged cache: a page or sequence number that the call cannot use
+    YSCV_DEV_NO_PAGE = 5,       // paged cache: no free page left
 };
 
 struct yscv_cuda_ctx {

@@ -1,0 +1,655 @@
+// Attention of ragged rows over a paged 8-bit cache, for the single tokens and short drafts of a decode step.
+//
+// With q = a_q n_q (n_q whole numbers of 24 bits, a row's largest at 8355711), k = s_k n_k and v = s_v n_v as the cache holds them,
+//   scores   q k = a_q s_k sum n_q n_k          n_q = 65536 q2 + 256 q1 + q0, digits in [-128, 127]
+//   output   p v = (s_v / 2^23) sum n_p n_v     n_p = p 2^23 of the softmax weights p <= 1 of a step, bytes p2 p1 p0
+// so both contractions are integer tensor-core products (mma.sync m16n8k32, int32 sums, exact) on the cache's bytes as they lie:
+// nothing is converted or transposed. Against two fp16 terms per operand, which the framework's other int8 cache takes, that is
+// three or two products for two and no conversion of the cache, which there is most of what the kernel issues. What is rounded: the
+// query to 2^-23 of its row's largest, a weight to 2^-24 of its step's largest, and fp32 sums over steps.
+//
+// Work: a step is 64 keys of a (sequence, KV head, block of R (position, head) pairs). All steps of a call are laid end to
+// end, sequence after sequence, and every warp of the GPU takes an equal run of them, so that neither one long conversation nor
+// many short ones leave SMs idle, whatever the lengths, which only the device knows. A warp is alone: it fetches its own keys and
+// values (bulk copies, two or three steps deep), keeps its own running maximum, sum and output, and writes a segment's result, or, where
+// the segment goes on in another warp, a record that kv_attention_merge_kernel adds to the others. No barrier joins warps.
+//
+// R = 8: the 16 rows of a product hold two digits of eight pairs, two products per tile instead of three.
+// Bound: the cache's bytes from HBM.
+#include <cfloat>
+
+#include "kv_pool.cuh"
+#include "tma.cuh"
+
+namespace yscv {
+
+constexpr int KA_STEP = 64;                   // keys of a step
+constexpr float KA_Q = 8355711.0f;            // 127 * (65536 + 256 + 1)
+constexpr float KA_P = 8388607.0f;            // 2^23 - 1
+constexpr float KA_MAGIC = 12582912.0f;       // 1.5 * 2^23: a sum that starts at its bits is the float MAGIC + sum (|sum| < 2^22)
+constexpr int KA_MAGIC_BITS = 0x4B400000;
+
+struct KvAttention {
+    KvLayer l;
+    const float *q;
+    float *out;
+    size_t q_stride, out_stride;
+    const int32_t *offsets, *start;
+    int n_q, group, causal, wide;
+    int window;                               // 0: none
+    float scale;                              // times log2(e)
+    long long *plan;                          // [0] steps, [1] steps of a warp, [2 ..] steps in front of a sequence
+    float *records;
+    int *status;
+};
+
+template <int D> struct KaGeom {
+    static constexpr int WARPS = D == 64 ? 8 : D == 128 ? 6 : 3, STAGES = D == 64 ? 3 : 2;
+    static constexpr int TILE = KA_STEP * D, STAGE = 2 * TILE;
+    static constexpr int WARP_BYTES = STAGES * STAGE + STAGES * 32 + 32;   // tiles, scales, barriers
+    static constexpr int RECORD_ROW = D + 2;
+};
+
+// A sequence's part of a call
+struct KaSeq {
+    int start, rows, lo, steps, blocks;       // lo: first key that any row sees, at a step's border
+};
+__device__ __forceinline__ KaSeq ka_seq(const KvAttention &a, int start, int rows, int R) {
+    KaSeq s;
+    s.start = start;
+    s.rows = start < 0 ? 0 : max(rows, 0);
+    s.lo = a.window > 0 ? max(0, start + 1 - a.window) & ~(KA_STEP - 1) : 0;
+    s.steps = s.rows > 0 ? (int)(((long long)start + s.rows - s.lo + KA_STEP - 1) / KA_STEP) : 0;
+    s.blocks = (int)(((long long)s.rows * a.group + R - 1) / R);
+    return s;
+}
+
+// D = A B + C: C the sums so far, or, for the first product, MAGIC's bits
+#define KA_MMA(name, type)                                                                                                              \
+    __device__ __forceinline__ void name(int (&d)[4], const uint32_t (&x)[4], uint32_t b0, uint32_t b1, bool first) {                   \
+        if (first)                                                                                                                      \
+            asm("mma.sync.aligned.m16n8k32.row.col.s32." type ".s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"    \
+                : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                                        \
+                : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1), "r"(KA_MAGIC_BITS));                                    \
+        else                                                                                                                            \
+            asm("mma.sync.aligned.m16n8k32.row.col.s32." type ".s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"        \
+                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                                        \
+                : "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(b0), "r"(b1));                                                        \
+    }
+KA_MMA(ka_mma_s8, "s8")
+KA_MMA(ka_mma_u8, "u8")
+#undef KA_MMA
+__device__ __forceinline__ void ka_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float ka_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float ka_sum(int bits) { return __int_as_float(bits) - KA_MAGIC; }
+
+// Steps in front of every sequence, into shared memory, by all threads; returns the steps of the call
+__device__ __forceinline__ long long ka_plan(const KvAttention &a, int R, long long *cum, int2 *info, long long *sums, int threads) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.l.n_seq;
+    const int per = (n + threads - 1) / threads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) {
+        const int row0 = a.offsets[i];
+        int2 v = make_int2(a.start[i], a.offsets[i + 1] - row0);
+        const KaSeq s = ka_seq(a, v.x, v.y, R);
+        info[i] = v;
+        cum[i] = mine;
+        mine += (long long)s.steps * s.blocks * a.l.n_kv;
+    }
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    long long before = x - mine, total = 0;
+    for (int w = 0; w < threads / 32; ++w) {
+        if (w < warp) before += sums[w];
+        total += sums[w];
+    }
+    for (int i = i0; i < i1; ++i) cum[i] += before;
+    if (tid == 0) cum[n] = total;
+    __syncthreads();
+    return total;
+}
+
+// Where a warp is in the steps of the call
+struct KaWalk {
+    int seq, head, block, step;
+    KaSeq s;
+    __device__ void load(const KvAttention &a, const int2 *info, int R) { s = ka_seq(a, info[seq].x, info[seq].y, R); }
+    __device__ void seek(const KvAttention &a, const long long *cum, const int2 *info, int R, long long u) {
+        int lo = 0, hi = a.l.n_seq;
+        while (hi - lo > 1) {
+            const int m = (lo + hi) >> 1;
+            if (cum[m] <= u) lo = m;
+            else hi = m;
+        }
+        seq = lo;
+        load(a, info, R);
+        const long long r = u - cum[seq], segment = r / s.steps;
+        step = (int)(r - segment * s.steps);
+        head = (int)(segment / s.blocks);
+        block = (int)(segment - (long long)head * s.blocks);
+    }
+    // the next step of the call (there is one)
+    __device__ void next(const KvAttention &a, const int2 *info, int R) {
+        if (++step < s.steps) return;
+        step = 0;
+        if (++block < s.blocks) return;
+        block = 0;
+        if (++head < a.l.n_kv) return;
+        head = 0;
+        do {
+            ++seq;
+            load(a, info, R);
+        } while (s.rows == 0);
+    }
+};
+
+template <int D, int R>
+__global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(const __grid_constant__ KvAttention a) {
+    using G = KaGeom<D>;
+    constexpr int NR = R / 8, KS = D / 32, NT = D / 8, STAGES = G::STAGES, THREADS = G::WARPS * 32;
+    constexpr int TERMS = R == 8 ? 2 : 3;     // products per tile and 32 of the contraction
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ long long sums[G::WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    unsigned char *mine = smem + warp * (STAGES * G::STAGE);
+    float *scales = reinterpret_cast<float *>(smem + G::WARPS * STAGES * G::STAGE) + warp * STAGES * 8;
+    const uint32_t bars = smem_u32(smem) + G::WARPS * (STAGES * G::STAGE + STAGES * 32) + warp * 32;
+    long long *cum = reinterpret_cast<long long *>(smem + G::WARPS * G::WARP_BYTES);
+    int2 *info = reinterpret_cast<int2 *>(cum + a.l.n_seq + 1);
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(bars + i * 8, 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    pdl_wait();
+    pdl_trigger();
+    const long long total = ka_plan(a, R, cum, info, sums, THREADS);
+    // consecutive runs lie on different SMs
+    const long long w = (long long)warp * gridDim.x + blockIdx.x, warps = (long long)gridDim.x * G::WARPS;
+    const long long share = (total + warps - 1) / warps;
+    if (blockIdx.x == 0) {
+        for (int i = tid; i <= a.l.n_seq; i += THREADS) a.plan[2 + i] = cum[i];
+        if (tid == 0) { a.plan[0] = total; a.plan[1] = share; }
+    }
+    const long long u0 = w * share, u1 = min(total, u0 + share);
+    if (u0 >= u1) return;
+    const int n = (int)(u1 - u0);
+
+    // ---- fetching: lane i < 4 looks after the step's i-th group of 16 keys ----
+    KaWalk f;
+    f.seek(a, cum, info, R, u0);
+    int ahead = 0, next_id;                   // steps fetched; the page of this lane's group in the next one
+    auto groups_of = [&](const KaWalk &x) { return min(4, (x.s.start + x.s.rows - (x.s.lo + x.step * KA_STEP) + KV_GROUP - 1) / KV_GROUP); };
+    auto page_of = [&](const KaWalk &x) {
+        int id = -1;
+        if (lane < groups_of(x)) {
+            const int at = (x.s.lo + x.step * KA_STEP + KV_GROUP * lane) >> a.l.page_shift;
+            if (at < a.l.max_pages) id = __ldg(a.l.table + (size_t)x.seq * a.l.max_pages + at);
+            if (at >= a.l.max_pages) atomicExch(a.status, YSCV_DEV_POS_OVERFLOW);
+            else if (id < 0 || id >= a.l.n_pages) { id = -1; atomicExch(a.status, YSCV_DEV_BAD_NUMBER); }
+        }
+        return id;
+    };
+    const int piece = min(a.l.page, KA_STEP) / KV_GROUP;   // groups that lie together
+    auto fetch = [&]() {
+        const int st = ahead % STAGES, id = next_id;
+        const uint32_t bar = bars + st * 8, to = smem_u32(mine) + st * G::STAGE;
+        const unsigned there = __ballot_sync(0xffffffffu, id >= 0);
+        if (lane == 0) mbar_expect_tx(bar, __popc(there) * (2 * KV_GROUP * D));
+        __syncwarp();
+        if (lane < 4) {
+            const uint32_t sc = smem_u32(scales + st * 8 + lane);
+            if (id >= 0) {
+                const size_t s_at = (size_t)id * a.l.n_kv + f.head;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(sc), "l"(a.l.ks + s_at) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(sc + 16), "l"(a.l.vs + s_at) : "memory");
+                if (lane % piece == 0) {
+                    const int groups = min(piece, groups_of(f) - lane);
+                    const size_t at = kv_group_at(a.l, id, f.head, ((f.s.lo + f.step * KA_STEP + KV_GROUP * lane) & (a.l.page - 1)) / KV_GROUP);
+                    bulk_load(to + lane * (KV_GROUP * D), a.l.k + at, groups * KV_GROUP * D, bar);
+                    bulk_load(to + G::TILE + lane * (KV_GROUP * D), a.l.v + at, groups * KV_GROUP * D, bar);
+                }
+            } else {
+                scales[st * 8 + lane] = 0.0f;
+                scales[st * 8 + 4 + lane] = -1.0f;       // no such keys
+            }
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        if (++ahead < n) {
+            f.next(a, info, R);
+            next_id = page_of(f);
+        }
+    };
+    next_id = page_of(f);
+    for (int i = 0; i < STAGES - 1; ++i) {
+        if (i < n) fetch();
+        else asm volatile("cp.async.commit_group;\n" ::: "memory");
+    }
+
+    KaWalk c;
+    c.seek(a, cum, info, R, u0);
+    uint32_t qa[KS][NR == 1 ? 6 : 12];        // the query's digits as operands
+    float qs[NR], m[NR], l[NR], o[NT][2 * NR];
+    int lim[NR], low[NR];
+    const int first = t < 2 ? 0 : 2;          // of its four tokens of a group, which two a thread has in the first tile
+    const uint32_t sel0 = t < 2 ? 0x5410u : 0x1054u, sel1 = t < 2 ? 0x7632u : 0x3276u;
+    // rows of ldmatrix: tokens 0,1,4,5,10,11,14,15 and 2,3,6,7,8,9,12,13 of a group: a thread then has tokens 4 t .. 4 t + 3, and the
+    // eight rows of a tile touch all banks
+    const int r8 = lane & 7, half = lane >> 4, tq = r8 >> 1;
+    const int token = 4 * tq + ((tq >> 1) ^ half) * 2 + (r8 & 1);
+    const uint32_t k_lane = ((lane >> 3) & 1) * 256 + token * 16;
+    const uint32_t v_lane = ((lane >> 3) & 1) * (KV_GROUP * D) + ((lane >> 4) * 8 + r8) * 16;
+
+    bool begin = true, alive = true;
+    for (int i = 0; i < n; ++i) {
+        __syncwarp();                          // every lane is done with the stage that is filled now
+        if (i + STAGES - 1 < n) fetch();
+        else asm volatile("cp.async.commit_group;\n" ::: "memory");
+        const int key0 = c.s.lo + c.step * KA_STEP;
+        if (begin) {
+            begin = false;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int pair = c.block * R + 8 * r + g, s = pair / a.group;
+                const bool live = pair < c.s.rows * a.group;
+                lim[r] = !live ? 0 : a.causal ? c.s.start + s + 1 : c.s.start + c.s.rows;
+                low[r] = a.window > 0 ? c.s.start + s + 1 - a.window : 0;
+                const float *src = a.q + (size_t)(a.offsets[c.seq] + (live ? s : 0)) * a.q_stride + (size_t)(c.head * a.group + (live ? pair - s * a.group : 0)) * D;
+                float x[KS][8], most = 0.0f, bad = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float *p = src + 32 * k + 16 * h + 4 * t;
+                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (live) y = a.wide ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+                        x[k][4 * h] = y.x; x[k][4 * h + 1] = y.y; x[k][4 * h + 2] = y.z; x[k][4 * h + 3] = y.w;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        most = fmaxf(most, fabsf(x[k][j]));
+                        bad = fmaf(x[k][j], 0.0f, bad);
+                    }
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                    bad += __shfl_xor_sync(0xffffffffu, bad, d);
+                }
+                most = fminf(fmaxf(most, KV_LEAST), FLT_MAX);
+                const float up = __fdiv_rn(KA_Q, most);
+                qs[r] = __fdiv_rn(most, KA_Q) * a.scale + bad;   // (bad: 0, or NaN)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t dig[3][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        dig[0][h] = dig[1][h] = dig[2][h] = 0u;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int v = __float2int_rn(fminf(fmaxf(x[k][4 * h + j] * up, -KA_Q), KA_Q));
+                            const int d0 = (int)(int8_t)v, v1 = (v - d0) >> 8, d1 = (int)(int8_t)v1, d2 = (v1 - d1) >> 8;
+                            dig[0][h] |= (uint32_t)(d0 & 255) << (8 * j);
+                            dig[1][h] |= (uint32_t)(d1 & 255) << (8 * j);
+                            dig[2][h] |= (uint32_t)(d2 & 255) << (8 * j);
+                        }
+                    }
+                    if constexpr (NR == 1) {   // {q2, q1} in one operand, {q0, 0} in the other
+                        qa[k][0] = dig[2][0]; qa[k][1] = dig[1][0]; qa[k][2] = dig[2][1]; qa[k][3] = dig[1][1];
+                        qa[k][4] = dig[0][0]; qa[k][5] = dig[0][1];
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < 3; ++d) { qa[k][4 * d + r] = dig[2 - d][0]; qa[k][4 * d + 2 + r] = dig[2 - d][1]; }
+                    }
+                }
+                m[r] = -INFINITY;
+                l[r] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 2 * NR; ++e) o[j][e] = 0.0f;
+        }
+        const int st = i % STAGES;
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 1) : "memory");
+        alive = mbar_wait(bars + st * 8, (uint32_t)(i / STAGES) & 1u, a.status);
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        const uint32_t ks_at = smem_u32(mine) + st * G::STAGE, vs_at = ks_at + G::TILE;
+        const float4 ksc = *reinterpret_cast<const float4 *>(scales + st * 8), vsc = *reinterpret_cast<const float4 *>(scales + st * 8 + 4);
+        const float kscale[4] = {ksc.x, ksc.y, ksc.z, ksc.w}, vscale[4] = {vsc.x, vsc.y, vsc.z, vsc.w};
+        // ---- scores ----
+        float s[NR][16];                       // [row][4 group + token of the thread], tile order
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp) {
+            int acc[2][TERMS][4];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t b[4];
+                ka_ldmatrix(b, ks_at + grp * (KV_GROUP * D) + k * 512 + k_lane);
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    if constexpr (NR == 1) {
+                        const uint32_t x1[4] = {qa[k][0], qa[k][1], qa[k][2], qa[k][3]}, x0[4] = {qa[k][4], 0u, qa[k][5], 0u};
+                        ka_mma_s8(acc[tile][0], x1, b[2 * tile], b[2 * tile + 1], k == 0);
+                        ka_mma_s8(acc[tile][1], x0, b[2 * tile], b[2 * tile + 1], k == 0);
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < 3; ++d) {
+                            const uint32_t x[4] = {qa[k][4 * d], qa[k][4 * d + 1], qa[k][4 * d + 2], qa[k][4 * d + 3]};
+                            ka_mma_s8(acc[tile][d], x, b[2 * tile], b[2 * tile + 1], k == 0);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        const float d2 = ka_sum(acc[tile][0][2 * r + e]);
+                        const float d1 = ka_sum(NR == 1 ? acc[tile][0][2 + e] : acc[tile][1][2 * r + e]);
+                        const float d0 = ka_sum(acc[tile][TERMS - 1][2 * r + e]);
+                        s[r][4 * grp + 2 * tile + e] = fmaf(d2, 65536.0f, fmaf(d1, 256.0f, d0)) * (qs[r] * kscale[grp]);
+                    }
+        }
+        bool edge = vscale[0] < 0.0f || vscale[1] < 0.0f || vscale[2] < 0.0f || vscale[3] < 0.0f;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) edge |= key0 + KA_STEP > lim[r] || key0 < low[r];
+        if (__any_sync(0xffffffffu, edge)) {
+#pragma unroll
+            for (int grp = 0; grp < 4; ++grp)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int key = key0 + 16 * grp + 4 * t + ((j & 2) ^ first) + (j & 1);
+#pragma unroll
+                    for (int r = 0; r < NR; ++r)
+                        if (key >= lim[r] || key < low[r] || vscale[grp] < 0.0f) s[r][4 * grp + j] = -INFINITY;
+                }
+        }
+        // ---- weights, relative to the step's own maximum ----
+        const float vmost = fmaxf(fmaxf(vscale[0], vscale[1]), fmaxf(vscale[2], vscale[3]));
+        float vc[4];
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp) vc[grp] = vscale[grp] > 0.0f ? fminf(__fdiv_rn(vscale[grp], vmost), 1.0f) * KA_P : 0.0f;
+        uint32_t pa[4][NR][3];                 // [group][row][digit, the highest first]
+        float w0[NR], alpha[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            float mx = s[r][0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[r][j]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float ref = mx == -INFINITY ? 0.0f : mx, m_new = fmaxf(m[r], mx);
+            float sum = 0.0f;
+#pragma unroll
+            for (int grp = 0; grp < 4; ++grp) {
+                uint32_t x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float p = ka_exp2(s[r][4 * grp + j] - ref);
+                    sum += p;
+                    x[j] = __float_as_uint(fmaf(p, vc[grp], 8388608.0f));   // 2^23 + n_p: the low bytes are the digits
+                }
+                const uint32_t y = __byte_perm(x[0], x[1], 0x5140), z = __byte_perm(x[2], x[3], 0x5140);
+                pa[grp][r][2] = __byte_perm(y, z, sel0);
+                pa[grp][r][1] = __byte_perm(y, z, sel1);
+                pa[grp][r][0] = __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), sel0);
+            }
+            alpha[r] = m_new == -INFINITY ? 1.0f : ka_exp2(m[r] - m_new);
+            const float beta = m_new == -INFINITY ? 0.0f : ka_exp2(mx - m_new);
+            l[r] = fmaf(l[r], alpha[r], beta * sum);
+            m[r] = m_new;
+            w0[r] = beta * (vmost > 0.0f ? vmost : 0.0f) * (1.0f / KA_P);
+        }
+        // ---- weighted values ----
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+            int acc[2][TERMS][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t b[4];
+                ka_ldmatrix(b, vs_at + k * (2 * KV_GROUP * D) + j * 128 + v_lane);
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    if constexpr (NR == 1) {
+                        const uint32_t x1[4] = {pa[2 * k][0][0], pa[2 * k][0][1], pa[2 * k + 1][0][0], pa[2 * k + 1][0][1]};
+                        const uint32_t x0[4] = {pa[2 * k][0][2], 0u, pa[2 * k + 1][0][2], 0u};
+                        ka_mma_u8(acc[tile][0], x1, b[2 * tile], b[2 * tile + 1], k == 0);
+                        ka_mma_u8(acc[tile][1], x0, b[2 * tile], b[2 * tile + 1], k == 0);
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < 3; ++d) {
+                            const uint32_t x[4] = {pa[2 * k][0][d], pa[2 * k][NR - 1][d], pa[2 * k + 1][0][d], pa[2 * k + 1][NR - 1][d]};
+                            ka_mma_u8(acc[tile][d], x, b[2 * tile], b[2 * tile + 1], k == 0);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float d2 = ka_sum(acc[tile][0][2 * r + e]);
+                        const float d1 = ka_sum(NR == 1 ? acc[tile][0][2 + e] : acc[tile][1][2 * r + e]);
+                        const float d0 = ka_sum(acc[tile][TERMS - 1][2 * r + e]);
+                        float &x = o[j + tile][2 * r + e];
+                        x = fmaf(d2, w0[r] * 65536.0f, fmaf(d1, w0[r] * 256.0f, fmaf(d0, w0[r], x * alpha[r])));
+                    }
+        }
+        // ---- the end of a segment, or of this warp's part of it ----
+        const bool last = c.step + 1 == c.s.steps;
+        if (last || i + 1 == n) {
+            const bool whole = last && i >= c.step;   // began here too
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                const int pair = c.block * R + 8 * r + g, sq = pair / a.group;
+                if (whole) {
+                    if (pair < c.s.rows * a.group) {
+                        const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+                        float *dst = a.out + (size_t)(a.offsets[c.seq] + sq) * a.out_stride + (size_t)(c.head * a.group + pair - sq * a.group) * D + 2 * t;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            if (a.wide) {
+                                *reinterpret_cast<float2 *>(dst + 8 * j) = make_float2(o[j][2 * r] * inv, o[j][2 * r + 1] * inv);
+                            } else {
+                                dst[8 * j] = o[j][2 * r] * inv;
+                                dst[8 * j + 1] = o[j][2 * r + 1] * inv;
+                            }
+                        }
+                    }
+                } else {
+                    // slot 2 w: the segment began in an earlier warp, 2 w + 1: here
+                    float *rec = a.records + ((size_t)(2 * w + (i >= c.step)) * R + 8 * r + g) * G::RECORD_ROW;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) *reinterpret_cast<float2 *>(rec + 8 * j + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+                    if (t == 0) *reinterpret_cast<float2 *>(rec + D) = make_float2(m[r], l[r]);
+                }
+            }
+            begin = true;
+        }
+        if (i + 1 < n) c.next(a, info, R);
+    }
+    if (!alive) {   // no copy may be in flight when the CTA leaves (bounded)
+        for (int j = max(0, ahead - STAGES); j < ahead; ++j) mbar_wait(bars + (j % STAGES) * 8, (uint32_t)(j / STAGES) & 1u, nullptr);
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+}
+
+// Adds the records of a segment that several warps shared: a CTA per (sequence, KV head) and pair
+template <int D, int R>
+__global__ void __launch_bounds__(128) kv_attention_merge_kernel(const __grid_constant__ KvAttention a) {
+    pdl_wait();
+    pdl_trigger();
+    constexpr int ROW = D + 2, PER = 128;
+    __shared__ float wt[PER], red[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seq = blockIdx.x, head = blockIdx.y;
+    const int row0 = a.offsets[seq];
+    const KaSeq s = ka_seq(a, a.start[seq], a.offsets[seq + 1] - row0, R);
+    if (s.steps == 0) return;
+    const long long share = a.plan[1], base = a.plan[2 + seq];
+    for (int pair = blockIdx.z; pair < s.rows * a.group; pair += gridDim.z) {
+        const int block = pair / R, r = pair - block * R;
+        const long long from = base + ((long long)head * s.blocks + block) * s.steps, to = from + s.steps;
+        const long long wa = from / share, wb = (to - 1) / share;
+        if (wa == wb) continue;                // one warp had it all and wrote it
+        const int parts = (int)(wb - wa) + 1;
+        auto record = [&](int p) { return a.records + ((size_t)(2 * (wa + p) + (p == 0)) * R + r) * ROW; };
+        float mx = -INFINITY;
+        for (int p = tid; p < parts; p += 128) mx = fmaxf(mx, record(p)[D]);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        if (lane == 0) red[warp] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        float sum = 0.0f, acc[D / 64] = {};
+        // D values by 128 threads: two threads a value at 64, each half of the records; two values a thread at 256
+        const int col = D == 64 ? tid & 63 : tid, odd = D == 64 ? tid >> 6 : 0, stride = D == 64 ? 2 : 1;
+        for (int p0 = 0; p0 < parts; p0 += PER) {
+            const int np = min(PER, parts - p0);
+            if (tid < np) {
+                const float2 ml = *reinterpret_cast<const float2 *>(record(p0 + tid) + D);
+                const float x = ka_exp2(ml.x - ref);
+                wt[tid] = x;
+                sum = fmaf(x, ml.y, sum);
+            }
+            __syncthreads();
+#pragma unroll 8
+            for (int p = odd; p < np; p += stride) {
+                const float *rec = record(p0 + p);
+#pragma unroll
+                for (int e = 0; e < (D == 256 ? 2 : 1); ++e) acc[e] = fmaf(wt[p], rec[col + 128 * e], acc[e]);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) red[4 + warp] = sum;
+        if (odd) wt[col] = acc[0];
+        __syncthreads();
+        sum = (red[4] + red[5]) + (red[6] + red[7]);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int sq = pair / a.group;
+        float *dst = a.out + (size_t)(row0 + sq) * a.out_stride + (size_t)(head * a.group + pair - sq * a.group) * D;
+        if (!odd) {
+            if (D == 64) acc[0] += wt[col];
+#pragma unroll
+            for (int e = 0; e < (D == 256 ? 2 : 1); ++e) dst[col + 128 * e] = acc[e] * inv;
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+static int ka_rows(size_t d, size_t pairs) { return d == 256 || pairs <= 8 ? 8 : 16; }
+
+static size_t ka_smem(size_t d, size_t n_seq) {
+    const size_t per = d == 64 ? KaGeom<64>::WARPS * KaGeom<64>::WARP_BYTES : d == 128 ? KaGeom<128>::WARPS * KaGeom<128>::WARP_BYTES
+                                                                                     : KaGeom<256>::WARPS * KaGeom<256>::WARP_BYTES;
+    return per + (n_seq + 1) * sizeof(long long) + n_seq * sizeof(int2);
+}
+static size_t ka_plan_bytes(size_t n_seq) { return (2 + n_seq + 1) * sizeof(long long) + 15 & ~(size_t)15; }
+static size_t ka_bytes(const yscv_cuda_ctx *ctx, size_t d, size_t n_seq, int R) {
+    const size_t warps = (size_t)ctx->sm_count * (d == 64 ? KaGeom<64>::WARPS : d == 128 ? KaGeom<128>::WARPS : KaGeom<256>::WARPS);
+    return ka_plan_bytes(n_seq) + 2 * warps * R * (d + 2) * sizeof(float);
+}
+
+template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttention &a, size_t pairs) {
+    auto kern = kv_attention_kernel<D, R>;
+    if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kern), ctx->device, 226 * 1024)) return rc;
+    YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KaGeom<D>::WARPS * 32), ka_smem(D, a.l.n_seq), ctx->stream, a));
+    ctx->launches++;
+    const unsigned z = (unsigned)(pairs < 1024 ? pairs : 1024);
+    YSCV_CUDA_TRY(launch_pdl(kv_attention_merge_kernel<D, R>, dim3((unsigned)a.l.n_seq, (unsigned)a.l.n_kv, z), dim3(128), 0, ctx->stream, a));
+    ctx->launches++;
+    YSCV_CUDA_TRY(cudaGetLastError());
+    ctx->last_kernel = "kv_block_attention(steps,imma)";
+    return YSCV_CUDA_OK;
+}
+
+static int ka_check(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows, size_t most_rows) {
+    if (!ctx) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null");
+    if (const int rc = kv_check_pool(pool)) return rc;
+    if (pool->d_head != 64 && pool->d_head != 128 && pool->d_head != 256)
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "attention takes heads of 64, 128 or 256, got %zu", pool->d_head);
+    if (n_q == 0 || n_q % pool->n_kv != 0) return fail(YSCV_CUDA_ERR_BAD_ARG, "n_q=%zu must be a positive multiple of n_kv=%zu", n_q, pool->n_kv);
+    if (n_q > 65535 || rows * n_q >= (1u << 31) || most_rows * n_q >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows or heads");
+    if (ka_smem(pool->d_head, pool->n_seq) > 226 * 1024)
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "attention takes pools of up to %zu sequences at this head size",
+                    (226 * 1024 - ka_smem(pool->d_head, 0)) / (sizeof(long long) + sizeof(int2)));
+    return YSCV_CUDA_OK;
+}
+
+}  // namespace yscv
+
+using namespace yscv;
+
+extern "C" {
+
+int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows, size_t most_rows,
+                                           size_t *bytes) {
+    if (const int rc = ka_check(ctx, pool, n_q, rows, most_rows)) return rc;
+    if (!bytes) return fail(YSCV_CUDA_ERR_BAD_ARG, "bytes is null");
+    *bytes = ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * (n_q / pool->n_kv)));
+    return YSCV_CUDA_OK;
+}
+
+int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_q, size_t q_stride,
+                                     size_t n_q, const int32_t *d_offsets, const int32_t *d_start, size_t rows, size_t most_rows, int causal,
+                                     size_t window, float scale, float *d_out, size_t out_stride, void *d_workspace, size_t workspace_bytes) {
+    if (const int rc = ka_check(ctx, pool, n_q, rows, most_rows)) return rc;
+    KvAttention a = {};
+    if (const int rc = kv_layer_of(pool, layer, &a.l)) return rc;
+    if (!d_q || !d_offsets || !d_start || !d_out || !d_workspace) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (q_stride < n_q * pool->d_head || out_stride < n_q * pool->d_head)
+        return fail(YSCV_CUDA_ERR_BAD_ARG, "a row stride is shorter than n_q * d_head");
+    if (!(scale >= 0.0f && scale <= FLT_MAX)) return fail(YSCV_CUDA_ERR_BAD_ARG, "scale must be 0 (the default) or positive");
+    if (reinterpret_cast<uintptr_t>(d_workspace) & 15) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the workspace must be 16-byte aligned");
+    const size_t group = n_q / pool->n_kv, pairs = most_rows * group;
+    const int R = ka_rows(pool->d_head, pairs);
+    const size_t need = ka_bytes(ctx, pool->d_head, pool->n_seq, R);
+    if (workspace_bytes < need) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
+    if (rows == 0 || most_rows == 0) return YSCV_CUDA_OK;
+    YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
+    a.q = d_q;
+    a.out = d_out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.offsets = d_offsets;
+    a.start = d_start;
+    a.n_q = (int)n_q;
+    a.group = (int)group;
+    a.causal = causal != 0;
+    a.window = (int)(window < (1u << 30) ? window : 0);
+    a.wide = ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15) == 0 && q_stride % 4 == 0 && out_stride % 4 == 0;
+    a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)pool->d_head)) * 1.4426950408889634f;
+    a.plan = static_cast<long long *>(d_workspace);
+    a.records = reinterpret_cast<float *>(static_cast<unsigned char *>(d_workspace) + ka_plan_bytes(pool->n_seq));
+    a.status = ctx->d_status;
+    switch (pool->d_head) {
+        case 64: return R == 8 ? ka_launch<64, 8>(ctx, a, pairs) : ka_launch<64, 16>(ctx, a, pairs);
+        case 128: return R == 8 ? ka_launch<128, 8>(ctx, a, pairs) : ka_launch<128, 16>(ctx, a, pairs);
+        default: return ka_launch<256, 8>(ctx, a, pairs);
+    }
+}
+
+}  // extern "C"

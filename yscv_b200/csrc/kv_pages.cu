@@ -1,0 +1,517 @@
+// Pages of a paged KV cache: which sequence has which (extend, trim, fork, compact), and the copies that follow.
+//
+// What is decided (who needs pages, which ones are free, what moves) is a few thousand integers and prefix sums in the order
+// of the sequences and of the pages: one block, so that no two launches have to agree on a count, bound by the latency of a dozen
+// dependent steps. What is moved (shared last pages, pages that close gaps) is bound by bytes, twice a page's in every layer:
+// kv_apply_kernel, behind it, reads how much there is from the workspace. Nothing comes back to the host.
+#include "kv_pool.cuh"
+
+namespace yscv {
+
+int kv_check_pool(const yscv_cuda_kv_pool *p) {
+    if (!p) return fail(YSCV_CUDA_ERR_BAD_ARG, "pool is null");
+    if (!p->d_k || !p->d_v || !p->d_kscale || !p->d_vscale || !p->d_refs || !p->d_table || !p->d_length)
+        return fail(YSCV_CUDA_ERR_BAD_ARG, "null array in the pool");
+    if (p->layers == 0 || p->n_pages == 0 || p->n_kv == 0 || p->d_head == 0 || p->n_seq == 0 || p->max_pages == 0)
+        return fail(YSCV_CUDA_ERR_BAD_ARG, "a size of the pool is zero");
+    if (p->page != 16 && p->page != 32 && p->page != 64 && p->page != 128)
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "pages hold 16, 32, 64 or 128 tokens, got %zu", p->page);
+    if (p->d_head % 16 != 0 || p->d_head > 256)
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "d_head %zu is not a multiple of 16 up to 256", p->d_head);
+    if (p->n_kv > 65535 || p->layers > 65535 || p->n_pages >= (1u << 30) || p->n_seq >= (1u << 20) || p->max_pages >= (1u << 24) ||
+        p->n_seq * p->max_pages >= (1u << 31) || p->max_pages * p->page >= (1u << 31))
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "a size of the pool is too large");
+    if ((reinterpret_cast<uintptr_t>(p->d_k) | reinterpret_cast<uintptr_t>(p->d_v)) & 15)
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "d_k and d_v must be 16-byte aligned");
+    return YSCV_CUDA_OK;
+}
+
+int kv_layer_of(const yscv_cuda_kv_pool *p, size_t layer, KvLayer *out) {
+    if (layer >= p->layers) return fail(YSCV_CUDA_ERR_BAD_ARG, "layer %zu of a pool with %zu", layer, p->layers);
+    const size_t heads = layer * p->n_pages * p->n_kv, bytes = heads * p->page * p->d_head;
+    out->k = p->d_k + bytes;
+    out->v = p->d_v + bytes;
+    out->ks = p->d_kscale + heads;
+    out->vs = p->d_vscale + heads;
+    out->table = p->d_table;
+    out->n_pages = (int)p->n_pages;
+    out->n_kv = (int)p->n_kv;
+    out->d = (int)p->d_head;
+    out->page = (int)p->page;
+    out->page_shift = p->page == 16 ? 4 : p->page == 32 ? 5 : p->page == 64 ? 6 : 7;
+    out->n_seq = (int)p->n_seq;
+    out->max_pages = (int)p->max_pages;
+    return YSCV_CUDA_OK;
+}
+
+constexpr int KVP_THREADS = 1024, KVP_WARPS = KVP_THREADS / 32;
+
+struct KvPages {
+    int32_t *refs, *table, *length;
+    int n_pages, n_seq, max_pages, page_shift;
+};
+
+// Workspace: how many copies (and pages in use), their sources and destinations, the free pages that are given out, where a
+// page went, the shared last page of a sequence
+struct KvWork {
+    int32_t *copies, *src, *dst, *free, *moved, *last;
+};
+static size_t kv_work_bytes(const yscv_cuda_kv_pool *p) {
+    const size_t list = p->n_seq > p->n_pages ? p->n_seq : p->n_pages;
+    return (16 + 2 * list + 2 * p->n_pages + p->n_seq) * sizeof(int32_t);
+}
+static KvWork kv_work_of(const yscv_cuda_kv_pool *p, void *ws) {
+    const size_t list = p->n_seq > p->n_pages ? p->n_seq : p->n_pages;
+    KvWork w;
+    w.copies = static_cast<int32_t *>(ws);
+    w.src = w.copies + 16;
+    w.dst = w.src + list;
+    w.free = w.dst + list;
+    w.moved = w.free + p->n_pages;
+    w.last = w.moved + p->n_pages;
+    return w;
+}
+
+// Exclusive prefix sum over the block's threads, and the sum of all
+__device__ __forceinline__ long long block_prefix(long long v, long long *shared, long long &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();   // (an earlier sum's readers are done)
+    if (lane == 31) shared[warp] = x;
+    __syncthreads();
+    long long before = 0;
+    total = 0;
+    for (int w = 0; w < KVP_WARPS; ++w) {
+        if (w < warp) before += shared[w];
+        total += shared[w];
+    }
+    return before + x - v;
+}
+
+// Pages [lo, hi) in order, a warp: list[at ..] gets those that are used (or free), up to `room` of the whole list
+__device__ __forceinline__ void list_pages(const int32_t *refs, int lo, int hi, bool used, int32_t *list, long long at, long long room) {
+    const int lane = threadIdx.x & 31;
+    for (int p0 = lo; p0 < hi && at < room; p0 += 128) {
+        bool take[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = p0 + 32 * i + lane;
+            take[i] = p < hi && (refs[p] > 0) == used;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned m = __ballot_sync(0xffffffffu, take[i]);
+            const long long to = at + __popc(m & ((1u << lane) - 1u));
+            if (take[i] && to < room) list[to] = p0 + 32 * i + lane;
+            at += __popc(m);
+        }
+    }
+}
+__device__ __forceinline__ int count_used(const int32_t *refs, int lo, int hi) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+#pragma unroll 8
+    for (int p = lo + lane; p < hi; p += 32) n += refs[p] > 0;
+    return __reduce_add_sync(0xffffffffu, n);
+}
+// A warp's run of the pages: whole pieces of 128, so that a list is written in order
+__device__ __forceinline__ void page_run(int n_pages, int &lo, int &hi) {
+    const int warp = threadIdx.x >> 5, per = ((n_pages + 127) / 128 + KVP_WARPS - 1) / KVP_WARPS * 128;
+    lo = min(warp * per, n_pages);
+    hi = min(lo + per, n_pages);
+}
+
+// ---- extend ---------------------------------------------------------------------------------------
+// Growth of a sequence but for its last page: tokens it has and gets, pages it has and will have
+struct KvGrowth {
+    int length, rows, held, wanted;
+    bool fits;
+};
+__device__ __forceinline__ KvGrowth growth_of(const KvPages &a, const int32_t *offsets, int i) {
+    KvGrowth g;
+    g.length = a.length[i];
+    g.rows = max(0, offsets[i + 1] - offsets[i]);
+    const int page = 1 << a.page_shift;
+    const long long end = (long long)g.length + g.rows;
+    g.fits = g.length >= 0 && end <= ((long long)a.max_pages << a.page_shift);
+    g.held = g.fits ? (g.length + page - 1) >> a.page_shift : 0;
+    g.wanted = g.fits ? (int)((end + page - 1) >> a.page_shift) : 0;
+    return g;
+}
+
+__global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a, const int32_t *__restrict__ offsets, int32_t *__restrict__ start,
+                                                                const KvWork w, int *__restrict__ status) {
+    __shared__ long long sums[KVP_WARPS];
+    __shared__ int copies;
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid == 0) copies = 0;
+    // what the sequences need, in their order: a thread takes a run of them
+    const int per = (a.n_seq + KVP_THREADS - 1) / KVP_THREADS, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
+    long long need = 0, wanted;
+    for (int i = i0; i < i1; ++i) {
+        const KvGrowth g = growth_of(a, offsets, i);
+        int last = -1;
+        if (g.rows > 0 && g.fits && (g.length & ((1 << a.page_shift) - 1))) {
+            const int p = a.table[(size_t)i * a.max_pages + g.held - 1];
+            if (p >= 0 && p < a.n_pages && a.refs[p] > 1) last = p;
+        }
+        w.last[i] = last;
+        if (g.rows > 0 && g.fits) need += g.wanted - g.held + (last >= 0);
+        if (g.rows > 0 && !g.fits) atomicExch(status, YSCV_DEV_POS_OVERFLOW);
+    }
+    const long long before = block_prefix(need, sums, wanted);
+    // the free pages, as many as are wanted, in their order
+    int lo, hi;
+    page_run(a.n_pages, lo, hi);
+    const int used = count_used(a.refs, lo, hi);
+    long long all_free;
+    const long long free_before = block_prefix(lane == 0 ? (hi - lo) - used : 0, sums, all_free);
+    list_pages(a.refs, lo, hi, false, w.free, __shfl_sync(0xffffffffu, free_before, 0), wanted < all_free ? wanted : all_free);
+    if (wanted > all_free && tid == 0) atomicExch(status, YSCV_DEV_NO_PAGE);
+    __syncthreads();   // the list is there, and nobody reads refs as they were any more
+    long long upto = before;
+    for (int i = i0; i < i1; ++i) {
+        const KvGrowth g = growth_of(a, offsets, i);
+        const int last = w.last[i];
+        long long at = upto;
+        const int mine = g.rows > 0 && g.fits ? g.wanted - g.held + (last >= 0) : 0;
+        upto += mine;
+        const bool ok = g.rows > 0 && g.fits && (mine == 0 || upto <= all_free);
+        start[i] = ok ? g.length : -1;
+        if (!ok) continue;
+        int32_t *row = a.table + (size_t)i * a.max_pages;
+        if (last >= 0) {
+            const int p = w.free[at++], k = atomicAdd(&copies, 1);
+            w.src[k] = last;
+            w.dst[k] = p;
+            row[g.held - 1] = p;
+            a.refs[p] = 1;
+            atomicSub(a.refs + last, 1);
+        }
+        for (int c = g.held; c < g.wanted; ++c) {
+            const int p = w.free[at++];
+            row[c] = p;
+            a.refs[p] = 1;
+        }
+        a.length[i] = g.length + g.rows;
+    }
+    __syncthreads();
+    if (tid == 0) *w.copies = copies;
+}
+
+// ---- compact --------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(KVP_THREADS) kv_compact_kernel(const KvPages a, const KvWork w) {
+    __shared__ long long sums[KVP_WARPS];
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31;
+    int lo, hi;
+    page_run(a.n_pages, lo, hi);
+    long long used;
+    const int all_used = count_used(a.refs, lo, hi);
+    block_prefix(lane == 0 ? all_used : 0, sums, used);
+    // gaps below `used`, and as many used pages from there on
+    const int mid = min(max((int)used, lo), hi);
+    long long gaps, above;
+    const int low_used = count_used(a.refs, lo, mid), high_used = count_used(a.refs, mid, hi);
+    const long long gap_at = block_prefix(lane == 0 ? (mid - lo) - low_used : 0, sums, gaps);
+    const long long above_at = block_prefix(lane == 0 ? high_used : 0, sums, above);
+    list_pages(a.refs, lo, mid, false, w.dst, __shfl_sync(0xffffffffu, gap_at, 0), gaps);
+    list_pages(a.refs, mid, hi, true, w.src, __shfl_sync(0xffffffffu, above_at, 0), above);
+    __syncthreads();
+    for (int k = tid; k < (int)gaps; k += KVP_THREADS) {
+        const int s = w.src[k], d = w.dst[k];
+        w.moved[s] = d;
+        a.refs[d] = a.refs[s];
+        a.refs[s] = 0;
+    }
+    if (tid == 0) { w.copies[0] = (int32_t)gaps; w.copies[1] = (int32_t)used; }
+}
+
+// ---- trim and fork: a warp per list entry ---------------------------------------------------------
+// The same sequence twice: an exchange gives a page to one of the two, the shorter length stays.
+__global__ void __launch_bounds__(256) kv_trim_kernel(const KvPages a, const int32_t *__restrict__ seqs, const int32_t *__restrict__ keep, int count,
+                                                      int *__restrict__ status) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < count; j += gridDim.x * 8) {
+        const int i = seqs[j];
+        if (i < 0 || i >= a.n_seq) {
+            if (lane == 0) atomicExch(status, YSCV_DEV_BAD_NUMBER);
+            continue;
+        }
+        int length = 0;
+        if (keep) {
+            if (lane == 0) {
+                const int k = max(0, keep[j]);
+                length = min(k, atomicMin(a.length + i, k));
+            }
+            length = max(0, __shfl_sync(0xffffffffu, length, 0));
+        } else if (lane == 0) {
+            a.length[i] = 0;
+        }
+        const int held = (int)(((long long)length + (1 << a.page_shift) - 1) >> a.page_shift);
+        int32_t *row = a.table + (size_t)i * a.max_pages;
+        for (int c = held + lane; c < a.max_pages; c += 32) {
+            if (row[c] < 0) continue;
+            const int p = atomicExch(row + c, -1);
+            if (p >= 0 && p < a.n_pages) atomicSub(a.refs + p, 1);
+        }
+    }
+}
+
+// The lists are looked through for a second use of a number, so that what is left out does not depend on timing
+__global__ void __launch_bounds__(256) kv_fork_kernel(const KvPages a, const int32_t *__restrict__ src, const int32_t *__restrict__ dst, int count,
+                                                      int *__restrict__ status) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < count; j += gridDim.x * 8) {
+        const int s = src[j], d = dst[j];
+        bool bad = s < 0 || s >= a.n_seq || d < 0 || d >= a.n_seq;
+        for (int o = lane; o < count; o += 32) bad |= dst[o] == s || (o < j && dst[o] == d);
+        bad = __any_sync(0xffffffffu, bad);
+        if (!bad) bad = a.length[d] != 0;   // (only this warp writes to d)
+        if (bad) {
+            if (lane == 0) atomicExch(status, YSCV_DEV_BAD_NUMBER);
+            continue;
+        }
+        const int length = min(max(0, a.length[s]), a.max_pages << a.page_shift);
+        const int held = (int)(((long long)length + (1 << a.page_shift) - 1) >> a.page_shift);
+        const int32_t *from = a.table + (size_t)s * a.max_pages;
+        int32_t *to = a.table + (size_t)d * a.max_pages;
+        for (int c = lane; c < held; c += 32) {
+            const int p = from[c];
+            to[c] = p;
+            if (p >= 0 && p < a.n_pages) atomicAdd(a.refs + p, 1);
+        }
+        __syncwarp();
+        if (lane == 0) a.length[d] = length;
+    }
+}
+
+// ---- what follows: copies of pages, positions of rows, page numbers that changed -------------------
+constexpr int KVP_PIECE = 16384;   // bytes a block copies at once: four loads of 16 in flight per thread
+
+struct KvApply {
+    unsigned char *k, *v;
+    float *ks, *vs;
+    size_t bytes;                  // of a page, keys or values
+    int n_kv, layers, n_pages, n_seq;
+    const int32_t *src, *dst, *copies;   // copies null: `count` of them
+    int count;
+    const int32_t *offsets, *start;      // null, or the positions of `rows` rows
+    int32_t *pos;
+    long long rows;
+    int32_t *table;                      // null, or the page numbers from copies[1] on become moved[]
+    const int32_t *moved;
+    long long entries;
+};
+
+__global__ void __launch_bounds__(256) kv_apply_kernel(const KvApply a, int *__restrict__ status) {
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x;
+    const int copies = a.copies ? a.copies[0] : a.count;
+    const long long thread = (long long)blockIdx.x * 256 + tid, threads = (long long)gridDim.x * 256;
+    if (a.pos) {
+        const int last = a.offsets[a.n_seq];
+        for (long long r = thread; r < a.rows; r += threads) {
+            int lo = 0, hi = a.n_seq;      // the last sequence whose rows begin at r or before
+            while (hi - lo > 1) {
+                const int m = (lo + hi) >> 1;
+                if (a.offsets[m] <= r) lo = m;
+                else hi = m;
+            }
+            const int p0 = r < last ? a.start[lo] : -1;
+            a.pos[r] = p0 < 0 ? -1 : p0 + (int)(r - a.offsets[lo]);
+        }
+    }
+    if (a.table) {
+        const int used = a.copies[1];
+        for (long long e = thread; copies > 0 && e < a.entries; e += threads) {
+            const int p = a.table[e];
+            if (p >= used && p < a.n_pages) a.table[e] = a.moved[p];
+        }
+    }
+    const int pieces = (int)((a.bytes + KVP_PIECE - 1) / KVP_PIECE);
+    const long long tasks = (long long)copies * a.layers * 2 * pieces;
+    for (long long t = blockIdx.x; t < tasks; t += gridDim.x) {
+        const int piece = (int)(t % pieces), which = (int)(t / pieces & 1);
+        const long long cl = t / pieces >> 1;
+        const int layer = (int)(cl % a.layers), c = (int)(cl / a.layers);
+        const int s = a.src[c], d = a.dst[c];
+        if (s < 0 || d < 0 || s == d) continue;
+        if (s >= a.n_pages || d >= a.n_pages) {
+            if (tid == 0) atomicExch(status, YSCV_DEV_BAD_NUMBER);
+            continue;
+        }
+        unsigned char *base = (which ? a.v : a.k) + (size_t)layer * a.n_pages * a.bytes;
+        const size_t at = (size_t)piece * KVP_PIECE, left = a.bytes - at;
+        const uint4 *from = reinterpret_cast<const uint4 *>(base + (size_t)s * a.bytes + at);
+        uint4 *to = reinterpret_cast<uint4 *>(base + (size_t)d * a.bytes + at);
+        const int n = (int)((left < KVP_PIECE ? left : KVP_PIECE) / 16);
+        uint4 x[KVP_PIECE / 4096];
+#pragma unroll
+        for (int i = 0; i < KVP_PIECE / 4096; ++i)
+            if (tid + 256 * i < n) x[i] = from[tid + 256 * i];
+#pragma unroll
+        for (int i = 0; i < KVP_PIECE / 4096; ++i)
+            if (tid + 256 * i < n) to[tid + 256 * i] = x[i];
+        if (piece == 0) {
+            float *scale = (which ? a.vs : a.ks) + (size_t)layer * a.n_pages * a.n_kv;
+            for (int h = tid; h < a.n_kv; h += 256) scale[(size_t)d * a.n_kv + h] = scale[(size_t)s * a.n_kv + h];
+        }
+    }
+}
+
+static KvPages pages_of(const yscv_cuda_kv_pool *p) {
+    KvPages a;
+    a.refs = p->d_refs;
+    a.table = p->d_table;
+    a.length = p->d_length;
+    a.n_pages = (int)p->n_pages;
+    a.n_seq = (int)p->n_seq;
+    a.max_pages = (int)p->max_pages;
+    a.page_shift = p->page == 16 ? 4 : p->page == 32 ? 5 : p->page == 64 ? 6 : 7;
+    return a;
+}
+static KvApply apply_of(const yscv_cuda_kv_pool *p) {
+    KvApply a = {};
+    a.k = reinterpret_cast<unsigned char *>(p->d_k);
+    a.v = reinterpret_cast<unsigned char *>(p->d_v);
+    a.ks = p->d_kscale;
+    a.vs = p->d_vscale;
+    a.bytes = p->n_kv * p->page * p->d_head;
+    a.n_kv = (int)p->n_kv;
+    a.layers = (int)p->layers;
+    a.n_pages = (int)p->n_pages;
+    a.n_seq = (int)p->n_seq;
+    return a;
+}
+static int launch_apply(yscv_cuda_ctx *ctx, const KvApply &a, size_t most_copies) {
+    const size_t pieces = (a.bytes + KVP_PIECE - 1) / KVP_PIECE, most = (size_t)8 * ctx->sm_count;
+    size_t blocks = most_copies * a.layers * 2 * pieces, others = (size_t)(a.rows > a.entries ? a.rows : a.entries) / 256 + 1;
+    if (blocks < others) blocks = others;
+    if (blocks > most) blocks = most;
+    YSCV_CUDA_TRY(launch_pdl(kv_apply_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a, ctx->d_status));
+    YSCV_CUDA_TRY(cudaGetLastError());
+    ctx->launches++;
+    return YSCV_CUDA_OK;
+}
+static int check_work(const yscv_cuda_kv_pool *p, const void *ws, size_t bytes) {
+    if (!ws) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace is null");
+    if (bytes < kv_work_bytes(p)) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", bytes, kv_work_bytes(p));
+    if (reinterpret_cast<uintptr_t>(ws) & 3) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the workspace must be 4-byte aligned");
+    return YSCV_CUDA_OK;
+}
+
+}  // namespace yscv
+
+using namespace yscv;
+
+#define KV_PROLOGUE(ctx, pool)                                             \
+    if (!(ctx)) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null");         \
+    if (const int rc_ = kv_check_pool(pool)) return rc_;                   \
+    YSCV_CUDA_TRY(cudaSetDevice((ctx)->device))
+
+extern "C" {
+
+int yscv_cuda_kv_pages_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t *bytes) {
+    if (!ctx || !bytes) return fail(YSCV_CUDA_ERR_BAD_ARG, "null argument");
+    if (const int rc = kv_check_pool(pool)) return rc;
+    *bytes = kv_work_bytes(pool);
+    return YSCV_CUDA_OK;
+}
+
+int yscv_cuda_kv_pages_extend_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_offsets, size_t rows,
+                                  int32_t *d_start, int32_t *d_pos, void *d_workspace, size_t workspace_bytes) {
+    KV_PROLOGUE(ctx, pool);
+    if (!d_offsets || !d_start || (rows > 0 && !d_pos)) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (rows >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows");
+    if (const int rc = check_work(pool, d_workspace, workspace_bytes)) return rc;
+    const KvWork w = kv_work_of(pool, d_workspace);
+    YSCV_CUDA_TRY(launch_pdl(kv_extend_kernel, dim3(1), dim3(KVP_THREADS), 0, ctx->stream, pages_of(pool), d_offsets, d_start, w, ctx->d_status));
+    YSCV_CUDA_TRY(cudaGetLastError());
+    ctx->launches++;
+    KvApply a = apply_of(pool);
+    a.src = w.src;
+    a.dst = w.dst;
+    a.copies = w.copies;
+    a.offsets = d_offsets;
+    a.start = d_start;
+    a.pos = d_pos;
+    a.rows = (long long)rows;
+    ctx->last_kernel = "kv_pages_extend";
+    return launch_apply(ctx, a, pool->n_seq);
+}
+
+int yscv_cuda_kv_pages_trim_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_seqs, const int32_t *d_keep,
+                                size_t count) {
+    KV_PROLOGUE(ctx, pool);
+    if (count == 0) return YSCV_CUDA_OK;
+    if (!d_seqs) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (count >= (1u << 30)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "list too long");
+    const unsigned blocks = (unsigned)((count + 7) / 8 < 4096 ? (count + 7) / 8 : 4096);
+    YSCV_CUDA_TRY(launch_pdl(kv_trim_kernel, dim3(blocks), dim3(256), 0, ctx->stream, pages_of(pool), d_seqs, d_keep, (int)count, ctx->d_status));
+    YSCV_CUDA_TRY(cudaGetLastError());
+    ctx->launches++;
+    ctx->last_kernel = "kv_pages_trim";
+    return YSCV_CUDA_OK;
+}
+
+int yscv_cuda_kv_pages_fork_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_src, const int32_t *d_dst,
+                                size_t count) {
+    KV_PROLOGUE(ctx, pool);
+    if (count == 0) return YSCV_CUDA_OK;
+    if (!d_src || !d_dst) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (count >= (1u << 20)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "list too long");
+    const unsigned blocks = (unsigned)((count + 7) / 8 < 4096 ? (count + 7) / 8 : 4096);
+    YSCV_CUDA_TRY(launch_pdl(kv_fork_kernel, dim3(blocks), dim3(256), 0, ctx->stream, pages_of(pool), d_src, d_dst, (int)count, ctx->d_status));
+    YSCV_CUDA_TRY(cudaGetLastError());
+    ctx->launches++;
+    ctx->last_kernel = "kv_pages_fork";
+    return YSCV_CUDA_OK;
+}
+
+int yscv_cuda_kv_pages_compact_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, void *d_workspace, size_t workspace_bytes) {
+    KV_PROLOGUE(ctx, pool);
+    if (const int rc = check_work(pool, d_workspace, workspace_bytes)) return rc;
+    const KvWork w = kv_work_of(pool, d_workspace);
+    YSCV_CUDA_TRY(launch_pdl(kv_compact_kernel, dim3(1), dim3(KVP_THREADS), 0, ctx->stream, pages_of(pool), w));
+    YSCV_CUDA_TRY(cudaGetLastError());
+    ctx->launches++;
+    KvApply a = apply_of(pool);
+    a.src = w.src;
+    a.dst = w.dst;
+    a.copies = w.copies;
+    a.table = pool->d_table;
+    a.moved = w.moved;
+    a.entries = (long long)(pool->n_seq * pool->max_pages);
+    ctx->last_kernel = "kv_pages_compact";
+    return launch_apply(ctx, a, pool->n_pages);
+}
+
+int yscv_cuda_kv_pages_copy_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_src, const int32_t *d_dst,
+                                size_t count) {
+    KV_PROLOGUE(ctx, pool);
+    if (count == 0) return YSCV_CUDA_OK;
+    if (!d_src || !d_dst) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (count >= (1u << 30)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "list too long");
+    KvApply a = apply_of(pool);
+    a.src = d_src;
+    a.dst = d_dst;
+    a.count = (int)count;
+    ctx->last_kernel = "kv_pages_copy";
+    return launch_apply(ctx, a, count);
+}
+
+}  // extern "C"

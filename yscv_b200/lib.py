@@ -136,6 +136,18 @@ SIGNATURES = {
                                                   _vp, _sz]),
     "yscv_cuda_gqa_attention_i8_dev": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp,
                                                  C.c_int, _vp]),
+    "yscv_cuda_rope_dev": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz]),
+    "yscv_cuda_kv_block_append_dev": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
+    "yscv_cuda_kv_block_read_dev": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
+    "yscv_cuda_kv_block_attention_workspace": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(_sz)]),
+    "yscv_cuda_kv_block_attention_dev": (C.c_int, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _sz, C.c_int, _sz, C.c_float,
+                                                   _vp, _sz, _vp, _sz]),
+    "yscv_cuda_kv_pages_workspace": (C.c_int, [_vp, _vp, C.POINTER(_sz)]),
+    "yscv_cuda_kv_pages_extend_dev": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp, _vp, _sz]),
+    "yscv_cuda_kv_pages_trim_dev": (C.c_int, [_vp, _vp, _vp, _vp, _sz]),
+    "yscv_cuda_kv_pages_fork_dev": (C.c_int, [_vp, _vp, _vp, _vp, _sz]),
+    "yscv_cuda_kv_pages_compact_dev": (C.c_int, [_vp, _vp, _vp, _sz]),
+    "yscv_cuda_kv_pages_copy_dev": (C.c_int, [_vp, _vp, _vp, _vp, _sz]),
 }
 
 WEIGHT_MATMUL_KN, WEIGHT_GEMM_NK, WEIGHT_GEMM_KN = 0, 1, 2
@@ -166,6 +178,33 @@ class DecodeLayer(C.Structure):
     """yscv_cuda_decode_layer."""
     _fields_ = [("qkv", _vp), ("o", _vp), ("gate_up", _vp), ("down", _vp), ("d_gamma_attn", _vp),
                 ("d_gamma_mlp", _vp), ("d_kcache", _vp), ("d_vcache", _vp), ("d_kscale", _vp), ("d_vscale", _vp)]
+
+
+class Rope(C.Structure):
+    """yscv_cuda_rope: how the pairs of a head turn. `scaling`: "none", "linear", "banded" or "yarn"."""
+    _fields_ = [("theta", C.c_double), ("rotary_dim", _sz), ("interleaved", C.c_int), ("scaling", C.c_int), ("factor", C.c_double),
+                ("original_positions", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double), ("low_band", C.c_double),
+                ("high_band", C.c_double), ("attention_factor", C.c_double)]
+
+    SCALINGS = ("none", "linear", "banded", "yarn")
+
+    def __init__(self, *, rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, scaling: str = "none",
+                 factor: float = 1.0, original_positions: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 low_band: float = 1.0, high_band: float = 4.0, attention_factor: float = 0.0):
+        if scaling not in self.SCALINGS:
+            raise ValueError(f"scaling {scaling!r} is none of {self.SCALINGS}")
+        super().__init__(theta, rotary_dim, int(bool(interleaved)), self.SCALINGS.index(scaling), factor, original_positions, beta_fast,
+                         beta_slow, low_band, high_band, attention_factor)
+
+
+class KvPool(C.Structure):
+    """yscv_cuda_kv_pool: a paged 8-bit KV cache in the caller's device memory (addresses as ints; layouts in the header)."""
+    _fields_ = [("d_k", _vp), ("d_v", _vp), ("d_kscale", _vp), ("d_vscale", _vp), ("layers", _sz), ("n_pages", _sz), ("n_kv", _sz),
+                ("d_head", _sz), ("page", _sz), ("d_refs", _vp), ("d_table", _vp), ("d_length", _vp), ("n_seq", _sz),
+                ("max_pages", _sz)]
+
+    def __init__(self, *, d_k, d_v, d_kscale, d_vscale, layers, n_pages, n_kv, d_head, page, d_refs, d_table, d_length, n_seq, max_pages):
+        super().__init__(d_k, d_v, d_kscale, d_vscale, layers, n_pages, n_kv, d_head, page, d_refs, d_table, d_length, n_seq, max_pages)
 
 
 def load_library():
@@ -795,6 +834,61 @@ class Context:
                                                         n_q, n_kv, d_head, max_seq, eps, rope_theta,
                                                         C.cast(C.byref(opt), _vp), C.byref(h)))
         return DecodePlan(self, h.value)
+
+    # -- sequences of different lengths: rotary positions and a paged 8-bit cache (device pointers) --
+    def rope_dev(self, d_x, x_stride, rows, n_heads, d_head, d_pos, rope: Rope, d_out, out_stride):
+        """Rotary positions of the first n_heads heads of every row; d_pos [rows], negative: a row that is left alone."""
+        _check(self.lib.yscv_cuda_rope_dev(self.handle, d_x, x_stride, rows, n_heads, d_head, d_pos, C.byref(rope), d_out, out_stride))
+
+    def kv_block_append_dev(self, pool: KvPool, layer, d_k, d_v, row_stride, d_offsets, d_start, most_rows):
+        """Keys and values of ragged rows into their pages (int8, one scale per page and KV head)."""
+        _check(self.lib.yscv_cuda_kv_block_append_dev(self.handle, C.byref(pool), layer, d_k, d_v, row_stride, d_offsets, d_start,
+                                                      most_rows))
+
+    def kv_block_read_dev(self, pool: KvPool, layer, d_offsets, d_start, most_rows, d_k_out, d_v_out, row_stride):
+        """The cached rows at the positions of a ragged call, as f32."""
+        _check(self.lib.yscv_cuda_kv_block_read_dev(self.handle, C.byref(pool), layer, d_offsets, d_start, most_rows, d_k_out, d_v_out,
+                                                    row_stride))
+
+    def kv_block_attention_workspace(self, pool: KvPool, n_q, rows, most_rows) -> int:
+        """Bytes of device memory a kv_block_attention_dev call needs."""
+        n = _sz()
+        _check(self.lib.yscv_cuda_kv_block_attention_workspace(self.handle, C.byref(pool), n_q, rows, most_rows, C.byref(n)))
+        return n.value
+
+    def kv_block_attention_dev(self, pool: KvPool, layer, d_q, q_stride, n_q, d_offsets, d_start, rows, most_rows, causal, window, scale,
+                               d_out, out_stride, d_workspace, workspace_bytes):
+        """Attention of ragged rows over their sequences' pages; window 0: none, scale 0: 1 / sqrt(d_head)."""
+        _check(self.lib.yscv_cuda_kv_block_attention_dev(self.handle, C.byref(pool), layer, d_q, q_stride, n_q, d_offsets, d_start, rows,
+                                                         most_rows, int(causal), window, scale, d_out, out_stride, d_workspace,
+                                                         workspace_bytes))
+
+    def kv_pages_workspace(self, pool: KvPool) -> int:
+        """Bytes of device memory kv_pages_extend_dev and kv_pages_compact_dev need."""
+        n = _sz()
+        _check(self.lib.yscv_cuda_kv_pages_workspace(self.handle, C.byref(pool), C.byref(n)))
+        return n.value
+
+    def kv_pages_extend_dev(self, pool: KvPool, d_offsets, rows, d_start, d_pos, d_workspace, workspace_bytes):
+        """Pages for the new rows of every sequence; d_start and d_pos receive where they go (-1: nowhere)."""
+        _check(self.lib.yscv_cuda_kv_pages_extend_dev(self.handle, C.byref(pool), d_offsets, rows, d_start, d_pos, d_workspace,
+                                                      workspace_bytes))
+
+    def kv_pages_trim_dev(self, pool: KvPool, d_seqs, d_keep, count):
+        """Sequences keep their first d_keep tokens (None: none) and give the pages behind them back."""
+        _check(self.lib.yscv_cuda_kv_pages_trim_dev(self.handle, C.byref(pool), d_seqs, d_keep, count))
+
+    def kv_pages_fork_dev(self, pool: KvPool, d_src, d_dst, count):
+        """Empty sequences d_dst share the pages of d_src."""
+        _check(self.lib.yscv_cuda_kv_pages_fork_dev(self.handle, C.byref(pool), d_src, d_dst, count))
+
+    def kv_pages_compact_dev(self, pool: KvPool, d_workspace, workspace_bytes):
+        """The used pages move to the lowest numbers."""
+        _check(self.lib.yscv_cuda_kv_pages_compact_dev(self.handle, C.byref(pool), d_workspace, workspace_bytes))
+
+    def kv_pages_copy_dev(self, pool: KvPool, d_src, d_dst, count):
+        """Page d_dst[j] becomes what page d_src[j] is, in every layer."""
+        _check(self.lib.yscv_cuda_kv_pages_copy_dev(self.handle, C.byref(pool), d_src, d_dst, count))
 
     def int4_from_matmulnbits_dev(self, d_src: int, d_dst: int, nbytes: int):
         _check(self.lib.yscv_cuda_int4_from_matmulnbits_dev(self.handle, _vp(d_src), _vp(d_dst), nbytes))
