@@ -277,6 +277,35 @@ def test_attention_of_a_few_rows(d, page, n_kv, group, start, counts, causal, wi
     ctx.close()
 
 
+PROMPTS = [
+    # d, page, n_kv, group, start, counts
+    (128, 64, 2, 8, [0], [300]),                       # whole tiles and a part of one
+    (64, 16, 1, 4, [0, 130, -1], [129, 33, 40]),       # positions around the tiles' borders
+    (128, 128, 1, 1, [5, 0], [257, 1]),                # one head a KV head: 256 positions to a tile
+    (64, 32, 2, 48, [700], [5]),                       # two positions of 48 heads to a half
+    (128, 16, 1, 128, [3, 1000], [3, 2]),              # one position to a half
+    (128, 32, 8, 6, [0, 2000, 17, 5], [31, 90, 0, 11]),
+    (64, 64, 4, 3, [64, 63], [200, 350]),
+    (128, 64, 1, 16, [9000], [20]),                    # a short piece over a long cache: every SM has a part of it
+]
+
+
+@pytest.mark.parametrize("d,page,n_kv,group,start,counts", PROMPTS)
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 100), (False, 33)])
+def test_attention_of_prompts(d, page, n_kv, group, start, counts, causal, window):
+    ctx = _context()
+    total = [max(0, s) + m for s, m in zip(start, counts)]
+    pool = Pool(ctx, layers=2, n_pages=sum(-(-t // page) for t in total) + 3, n_kv=n_kv, d=d, page=page, n_seq=len(start),
+                max_pages=-(-max(total) // page) + 1, seed=page)
+    pool.give(total)
+    q = torch.randn(sum(counts), n_kv * group, d, device="cuda", generator=pool.g)
+    got, live = _attend(ctx, pool, q, counts, start, causal, window, layer=1, pad=(n_kv % 2) * 3, shift=n_kv % 3)
+    assert "tcgen05" in ctx.last_kernel()
+    _done(ctx)
+    _check(got, live, *attention(pool, q, start, counts, causal, window, layer=1))
+    ctx.close()
+
+
 @pytest.mark.parametrize("size,scale", [(0.0, 0.0), (1e-30, 0.0), (30.0, 0.0), (1.0, 0.02), (1e30, 1e-30)])
 def test_attention_of_queries_of_any_size(size, scale):
     """Flat and peaked weights, rows whose size differs by 10^3, scales of pages that differ by 10^4."""
@@ -288,21 +317,23 @@ def test_attention_of_queries_of_any_size(size, scale):
     pool.give([s + m for s, m in zip(start, counts)])
     q = torch.randn(3, 8, 128, device="cuda", generator=pool.g) * size
     q[1:] *= torch.logspace(-3, 0, 8, device="cuda")[None, :, None]
-    got, live = _attend(ctx, pool, q, counts, start, scale=scale)
-    _done(ctx)
-    _check(got, live, *attention(pool, q, start, counts, scale=scale))
+    for most in (2, 100):   # the kernel for a few rows, and the one for prompts
+        got, live = _attend(ctx, pool, q, counts, start, scale=scale, most=most)
+        assert ("tcgen05" in ctx.last_kernel()) == (most == 100)
+        _done(ctx)
+        _check(got, live, *attention(pool, q, start, counts, scale=scale))
     ctx.close()
 
 
-@pytest.mark.parametrize("d", [64, 128, 256])
-def test_attention_keeps_rows_apart_that_are_no_numbers(d):
+@pytest.mark.parametrize("d,most", [(64, 3), (128, 3), (256, 3), (64, 90), (128, 90)])
+def test_attention_keeps_rows_apart_that_are_no_numbers(d, most):
     ctx = _context()
     pool = Pool(ctx, n_pages=40, n_kv=2, d=d, page=32, n_seq=2, max_pages=30)
     pool.give([501, 303])
     q = torch.randn(4, 8, d, device="cuda", generator=pool.g)
     clean = q.clone()
     q[0, 3, 5], q[2, 1, 0], q[2, 7, d - 1] = float("nan"), float("inf"), -float("inf")
-    got, live = _attend(ctx, pool, q, [1, 3], [500, 300])
+    got, live = _attend(ctx, pool, q, [1, 3], [500, 300], most=most)
     _done(ctx)
     want, tol = attention(pool, clean, [500, 300], [1, 3])
     bad = torch.zeros(4, 8, dtype=torch.bool, device="cuda")
@@ -312,28 +343,29 @@ def test_attention_keeps_rows_apart_that_are_no_numbers(d):
     ctx.close()
 
 
-def test_attention_leaves_pages_out_that_are_not_there():
+@pytest.mark.parametrize("most", [1, 80])
+def test_attention_leaves_pages_out_that_are_not_there(most):
     """A page number outside the pool hides its keys and is told; so are positions behind the table."""
     ctx = _context()
     pool = Pool(ctx, n_pages=30, n_kv=1, d=64, page=16, n_seq=2, max_pages=8)
     pool.give([100, 90])
     q = torch.randn(2, 4, 64, device="cuda", generator=pool.g)
-    good, _ = _attend(ctx, pool, q, [1, 1], [99, 89])
+    good, _ = _attend(ctx, pool, q, [1, 1], [99, 89], most=most)
     _done(ctx)
     for number in (-1, 30, 1 << 30, -(1 << 31)):
         pool.table[0, 2] = number
-        got, _ = _attend(ctx, pool, q, [1, 1], [99, 89])
+        got, _ = _attend(ctx, pool, q, [1, 1], [99, 89], most=most)
         _done(ctx, 4)
         assert torch.equal(got[1], good[1])
         k, v = (torch.cat([x[:32], x[48:100]]) for x in _rows_without(pool))
         want = torch.softmax(torch.einsum("hd,kd->hk", q[0].double(), k[:, 0]) / 8.0, -1) @ v[:, 0]
         assert float((got[0].double() - want).abs().max()) < 1e-5 * float(v.abs().max())   # (100 keys: 2^-18 + scores of 6)
     pool.table[0, 2] = 0
-    got, _ = _attend(ctx, pool, q, [1, 1], [8 * 16 + 40, 89])
+    got, _ = _attend(ctx, pool, q, [1, 1], [8 * 16 + 40, 89], most=most)
     assert ctx.device_status() in (3, 4)   # behind the table, and its last place has no page: the word holds either
     assert torch.equal(got[1], good[1])
     pool.table.fill_(-1)
-    got, _ = _attend(ctx, pool, q, [1, 1], [99, 89])
+    got, _ = _attend(ctx, pool, q, [1, 1], [99, 89], most=most)
     _done(ctx, 4)
     assert torch.all(got == 0)
     ctx.close()

@@ -18,7 +18,7 @@
 // Bound: the cache's bytes from HBM.
 #include <cfloat>
 
-#include "kv_pool.cuh"
+#include "kv_attention.cuh"
 #include "tma.cuh"
 
 namespace yscv {
@@ -28,20 +28,6 @@ constexpr float KA_Q = 8355711.0f;            // 127 * (65536 + 256 + 1)
 constexpr float KA_P = 8388607.0f;            // 2^23 - 1
 constexpr float KA_MAGIC = 12582912.0f;       // 1.5 * 2^23: a sum that starts at its bits is the float MAGIC + sum (|sum| < 2^22)
 constexpr int KA_MAGIC_BITS = 0x4B400000;
-
-struct KvAttention {
-    KvLayer l;
-    const float *q;
-    float *out;
-    size_t q_stride, out_stride;
-    const int32_t *offsets, *start;
-    int n_q, group, causal, wide;
-    int window;                               // 0: none
-    float scale;                              // times log2(e)
-    long long *plan;                          // [0] steps, [1] steps of a warp, [2 ..] steps in front of a sequence
-    float *records;
-    int *status;
-};
 
 template <int D> struct KaGeom {
     static constexpr int WARPS = D == 64 ? 8 : D == 128 ? 6 : 3, STAGES = D == 64 ? 3 : 2;
@@ -586,6 +572,11 @@ template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttenti
     return YSCV_CUDA_OK;
 }
 
+static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t group, size_t most_rows) {
+    return kv_prompt_takes(pool->d_head, pool->n_seq, group, most_rows) ? kv_prompt_bytes(ctx, pool->d_head, pool->n_seq)
+                                                                       : ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * group));
+}
+
 static int ka_check(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows, size_t most_rows) {
     if (!ctx) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null");
     if (const int rc = kv_check_pool(pool)) return rc;
@@ -609,7 +600,7 @@ int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_k
                                            size_t *bytes) {
     if (const int rc = ka_check(ctx, pool, n_q, rows, most_rows)) return rc;
     if (!bytes) return fail(YSCV_CUDA_ERR_BAD_ARG, "bytes is null");
-    *bytes = ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * (n_q / pool->n_kv)));
+    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, most_rows);
     return YSCV_CUDA_OK;
 }
 
@@ -626,7 +617,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     if (reinterpret_cast<uintptr_t>(d_workspace) & 15) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the workspace must be 16-byte aligned");
     const size_t group = n_q / pool->n_kv, pairs = most_rows * group;
     const int R = ka_rows(pool->d_head, pairs);
-    const size_t need = ka_bytes(ctx, pool->d_head, pool->n_seq, R);
+    const size_t need = attention_bytes(ctx, pool, group, most_rows);
     if (workspace_bytes < need) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     if (rows == 0 || most_rows == 0) return YSCV_CUDA_OK;
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
@@ -645,6 +636,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     a.plan = static_cast<long long *>(d_workspace);
     a.records = reinterpret_cast<float *>(static_cast<unsigned char *>(d_workspace) + ka_plan_bytes(pool->n_seq));
     a.status = ctx->d_status;
+    if (kv_prompt_takes(pool->d_head, pool->n_seq, group, most_rows)) return kv_prompt(ctx, a, d_workspace);
     switch (pool->d_head) {
         case 64: return R == 8 ? ka_launch<64, 8>(ctx, a, pairs) : ka_launch<64, 16>(ctx, a, pairs);
         case 128: return R == 8 ? ka_launch<128, 8>(ctx, a, pairs) : ka_launch<128, 16>(ctx, a, pairs);
