@@ -18,9 +18,10 @@
 // keys, 64 / 8 heads of 128, 507 us, a tile of 128 rows 6300 cycles.
 // Registers are moved between the warpgroups: 640 threads x 96 = 128 x (56 + 72 + 96 + 96 + 160).
 //
-// Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end and every SM takes an equal run; a segment that
-// several SMs share leaves records, which kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and
-// causal prompts need no order of CTAs.
+// Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, with room for KP_BEGIN tiles in front of each
+// segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
+// kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and causal prompts, whose first
+// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 456 us with tiles alone, 210 so; 276 with one, 212 with four).
 // Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128.
 #include <cfloat>
 
@@ -30,7 +31,7 @@
 
 namespace yscv {
 
-constexpr int KP_KEYS = 128, KP_ROWS = 128, KP_THREADS = 640, KP_NOTES = 8;
+constexpr int KP_KEYS = 128, KP_ROWS = 128, KP_THREADS = 640, KP_NOTES = 8, KP_BEGIN = 2;
 
 template <int D> struct KpGeom {
     static constexpr int OPERAND = KP_KEYS * D * 2, RAW = KP_KEYS * D;   // keys, or values, of a tile, in fp16 and as cached
@@ -145,10 +146,10 @@ __device__ __forceinline__ KpTile kp_tile(const KvAttention &a, int start, int r
     return t;
 }
 __device__ __forceinline__ int kp_tiles(int start, int rows, int QB) { return start < 0 || rows <= 0 ? 0 : (rows + QB - 1) / QB; }
-// Steps of the first `tiles` pairs tiles, a warp together
-__device__ __forceinline__ long long kp_steps(const KvAttention &a, int start, int rows, int QB, int tiles) {
+// Tiles of a sequence for one KV head, a warp together
+__device__ __forceinline__ long long kp_steps(const KvAttention &a, int start, int rows, int QB) {
     long long n = 0;
-    for (int q = threadIdx.x & 31; q < tiles; q += 32) n += kp_tile(a, start, rows, QB, q).steps;
+    for (int q = threadIdx.x & 31; q < kp_tiles(start, rows, QB); q += 32) n += kp_tile(a, start, rows, QB, q).steps;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
@@ -162,38 +163,45 @@ struct KpWalk {
         row0 = a.offsets[seq];
         rows = a.offsets[seq + 1] - row0;
     }
-    // a warp together
-    __device__ void seek(const KvAttention &a, const long long *cum, int QB, long long u) {
+    // The first tile at place u or behind it (u below the last place), a warp together. `at` [n_seq]: places in front of a sequence.
+    // Returns the tiles of the sequence in front of it; `gap`: places between u and it.
+    __device__ long long seek(const KvAttention &a, const long long *at, int QB, long long u, int &gap) {
         int lo = 0, hi = a.l.n_seq;
         while (hi - lo > 1) {
             const int m = (lo + hi) >> 1;
-            if (cum[m] <= u) lo = m;
+            if (at[m] <= u) lo = m;
             else hi = m;
         }
         seq = lo;
         load(a);
-        long long left = u - cum[seq];
+        long long left = u - at[seq], tiles = 0;
         const int lane = threadIdx.x & 31;
         for (int q0 = 0;; q0 += 32) {
-            const int n = q0 + lane < kp_tiles(start, rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps * a.l.n_kv : 0;
-            long long upto = n;
+            const int steps = q0 + lane < kp_tiles(start, rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps : 0;
+            const int n = steps > 0 ? (steps + KP_BEGIN) * a.l.n_kv : 0;
+            long long upto = n, tiles_upto = (long long)steps * a.l.n_kv;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
+                const long long y = __shfl_up_sync(0xffffffffu, upto, o), z = __shfl_up_sync(0xffffffffu, tiles_upto, o);
+                if (lane >= o) { upto += y; tiles_upto += z; }
             }
             const unsigned past = __ballot_sync(0xffffffffu, upto > left);
             if (past) {
-                const int at = __ffs(past) - 1;
-                left -= __shfl_sync(0xffffffffu, upto - n, at);
-                q = q0 + at;
+                const int f = __ffs(past) - 1;
+                left -= __shfl_sync(0xffffffffu, upto - n, f);
+                tiles += __shfl_sync(0xffffffffu, tiles_upto - (long long)steps * a.l.n_kv, f);
+                q = q0 + f;
                 break;
             }
             left -= __shfl_sync(0xffffffffu, upto, 31);
+            tiles += __shfl_sync(0xffffffffu, tiles_upto, 31);
         }
         t = kp_tile(a, start, rows, QB, q);
-        head = (int)(left / t.steps);
-        step = (int)(left - (long long)head * t.steps);
+        head = (int)(left / (t.steps + KP_BEGIN));
+        const int in = (int)(left - (long long)head * (t.steps + KP_BEGIN));
+        gap = max(0, KP_BEGIN - in);
+        step = max(0, in - KP_BEGIN);
+        return tiles + (long long)head * t.steps + step;
     }
     // the first step of the next segment (there is one)
     __device__ void next_segment(const KvAttention &a, int QB) {
@@ -227,7 +235,8 @@ template <int D>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvAttention a) {
     using G = KpGeom<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ long long sums[KP_THREADS / 32];
+    __shared__ longlong2 sums[KP_THREADS / 32];
+    __shared__ int run_tiles;
     __shared__ uint32_t tmem_slot;
     __shared__ int heads[KP_NOTES], begun[KP_NOTES];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -238,7 +247,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     const uint32_t raw_v_free = bars + 200, qstaged = bars + 208, qtaken = bars + 216, qfull = bars + 224, maxima = bars + 232;   // [2] by tile & 1
     float2 *stats = reinterpret_cast<float2 *>(smem + G::STATS);
     KpNote *notes = reinterpret_cast<KpNote *>(smem + G::NOTES);
-    long long *cum = reinterpret_cast<long long *>(smem + G::PLAN);
+    longlong2 *before = reinterpret_cast<longlong2 *>(smem + G::PLAN);     // [n_seq + 1] places, tiles
+    long long *cum = reinterpret_cast<long long *>(before + a.l.n_seq + 1); // [n_seq + 1] places
     const int group = a.group, QB = KP_ROWS / group;
 
     if (tid == 0) {
@@ -267,48 +277,59 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     }
     pdl_wait();
     pdl_trigger();
-    // ---- steps in front of every sequence ----
+    // ---- places and tiles in front of every sequence, and which are this CTA's ----
     for (int i = warp; i < a.l.n_seq; i += KP_THREADS / 32) {
         const int row0 = a.offsets[i], rows = a.offsets[i + 1] - row0, start = a.start[i];
-        const long long n = kp_steps(a, start, rows, QB, kp_tiles(start, rows, QB)) * a.l.n_kv;
-        if (lane == 0) cum[i] = n;
+        const long long n = kp_steps(a, start, rows, QB);
+        if (lane == 0) {
+            before[i].y = n * a.l.n_kv;
+            before[i].x = (n + (long long)KP_BEGIN * kp_tiles(start, rows, QB)) * a.l.n_kv;
+        }
     }
     __syncthreads();
     {
         const int n = a.l.n_seq, per = (n + KP_THREADS - 1) / KP_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-        long long mine = 0;
-        for (int i = i0; i < i1; ++i) mine += cum[i];
-        long long x = mine;
+        longlong2 mine = make_longlong2(0, 0);
+        for (int i = i0; i < i1; ++i) { mine.x += before[i].x; mine.y += before[i].y; }
+        longlong2 x = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            const long long y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
+            if (lane >= o) { x.x += y; x.y += z; }
         }
         if (lane == 31) sums[warp] = x;
         __syncthreads();
-        long long at = x - mine, total = 0;
-        for (int w = 0; w < KP_THREADS / 32; ++w) {
-            if (w < warp) at += sums[w];
-            total += sums[w];
-        }
+        longlong2 at = make_longlong2(x.x - mine.x, x.y - mine.y);
+        for (int w = 0; w < warp; ++w) { at.x += sums[w].x; at.y += sums[w].y; }
         for (int i = i0; i < i1; ++i) {
-            const long long c = cum[i];
-            cum[i] = at;
-            at += c;
+            const longlong2 c = before[i];
+            cum[i] = at.x;
+            before[i] = at;
+            at.x += c.x;
+            at.y += c.y;
         }
-        if (tid == 0) cum[n] = total;
+        if (tid == KP_THREADS - 1) { cum[n] = at.x; before[n] = at; }
     }
     at_fence_before();
     __syncthreads();
     at_fence_after();
     const uint32_t tmem = tmem_slot;
-    const long long total = cum[a.l.n_seq], share = (total + gridDim.x - 1) / gridDim.x;
+    const long long total = before[a.l.n_seq].x, share = (total + gridDim.x - 1) / gridDim.x;
     if (blockIdx.x == 0) {
         for (int i = tid; i <= a.l.n_seq; i += KP_THREADS) a.plan[2 + i] = cum[i];
         if (tid == 0) { a.plan[0] = total; a.plan[1] = share; }
     }
-    const long long u0 = min(total, blockIdx.x * share);
-    const int n = (int)(min(total, u0 + share) - u0);
+    const long long u0 = min(total, blockIdx.x * share), u1 = min(total, u0 + share);
+    if (warp == 0 && u0 < u1) {
+        KpWalk w;
+        int gap;
+        const long long t0 = w.seek(a, cum, QB, u0, gap) + before[w.seq].y;
+        const long long t1 = u1 < total ? w.seek(a, cum, QB, u1, gap) + before[w.seq].y : before[a.l.n_seq].y;
+        if (lane == 0) run_tiles = (int)(t1 - t0);
+    }
+    if (tid == 0 && u0 >= u1) run_tiles = 0;
+    __syncthreads();
+    const int n = run_tiles;
     // TMEM columns: queries (both terms), scores and then weights [2] x 128, weighted values
     const uint32_t t_q = tmem, t_s = tmem + 128, t_o = tmem + 384;
     auto par = [](int i) { return (uint32_t)(i >> 1) & 1u; };
@@ -371,7 +392,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
         } else if (warp == 1 && n > 0) {
             // ---- queries of the next segment, as they are: a copy a row, 16 bytes apart so that threads can read a row each ----
             KpWalk w;
-            w.seek(a, cum, QB, u0);
+            int gap;
+            w.seek(a, cum, QB, u0, gap);
             int i = 0, loaded = 1;
             for (int segment = 0;; ++segment) {
                 if (segment > 0) alive = __all_sync(0xffffffffu, kp_wait(qtaken, (uint32_t)(segment - 1) & 1u));
@@ -408,7 +430,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             const uint32_t full = values ? raw_v : raw_k, free = values ? raw_v_free : raw_k_free;
             const uint32_t to = base + (values ? G::RAW_V : G::RAW_K) + lane * (KV_GROUP * D);
             KpWalk w;
-            w.seek(a, cum, QB, u0);
+            int gap;
+            w.seek(a, cum, QB, u0, gap);
             const int piece = min(a.l.page / KV_GROUP, 8);        // groups that lie together, from a page's border on
             int id = -1;
             auto page = [&]() {
@@ -762,8 +785,10 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
     const long long total = a.plan[0], share = a.plan[1], border = (blockIdx.x + 1) * share;
     if (border >= total) return;
     KpWalk w;
-    w.seek(a, a.plan + 2, QB, border);
-    const long long from = border - w.step, to = from + w.t.steps;
+    int gap;
+    w.seek(a, a.plan + 2, QB, border, gap);
+    // places of the segment's first tile and of the end of its last
+    const long long from = border + gap - w.step, to = from + w.t.steps;
     if (w.step == 0 || from < border - share) return;      // no segment is cut here, or it was cut before
     const int s = w.q * QB + r / group;
     if (r >= QB * group || s >= w.rows) return;
@@ -800,7 +825,7 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * sizeof(long long); }
+static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * (sizeof(longlong2) + sizeof(long long)); }
 static size_t kp_plan_bytes(size_t n_seq) { return ((2 + n_seq + 1) * sizeof(long long) + 15) & ~(size_t)15; }
 
 size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head, size_t n_seq) {
