@@ -1,4 +1,5 @@
-// tcgen05 and fp16-splitting helpers of the prompt attention kernels (gqa_prefill_tc.cu, kv_block_prompt.cu).
+// tcgen05, fp16-splitting and two-at-a-time helpers of the attention kernels (gqa_prefill_tc.cu, kv_block_prompt.cu,
+// kv_block_attention.cu).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -74,6 +75,29 @@ __device__ __forceinline__ void at_split(float a, float b, uint32_t &hi, uint32_
     const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// ---- two floats at a time -------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t r, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 }  // namespace yscv

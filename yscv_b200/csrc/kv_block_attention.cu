@@ -11,13 +11,19 @@
 // Work: a step is 64 keys of a (sequence, KV head, block of R (position, head) pairs). All steps of a call are laid end to
 // end, sequence after sequence, and every warp of the GPU takes an equal run of them, so that neither one long conversation nor
 // many short ones leave SMs idle, whatever the lengths, which only the device knows. A warp is alone: it fetches its own keys and
-// values (bulk copies, two or three steps deep), keeps its own running maximum, sum and output, and writes a segment's result, or, where
-// the segment goes on in another warp, a record that kv_attention_merge_kernel adds to the others. No barrier joins warps.
+// values (bulk copies: the next step's keys under this one's softmax and values, its values under its scores), keeps its own running
+// maximum, sum and output, and writes a segment's result, or, where the segment goes on in another warp, a record that
+// kv_attention_merge_kernel adds to the others. No barrier joins warps.
+//
+// A step is a chain of some 1100 instructions, so what counts is how many warps an SM has, and their buffers: with two stages of both
+// operands and six warps at D = 128 the chain's latencies showed (64 sequences of 1000 to 8000 keys, 64 / 8 heads of 128: 133 us, IPC
+// 0.3 per scheduler); one place each for keys and values gives twelve.
 //
 // R = 8: the 16 rows of a product hold two digits of eight pairs, two products per tile instead of three.
 // Bound: the cache's bytes from HBM.
 #include <cfloat>
 
+#include "attention_tc.cuh"
 #include "kv_attention.cuh"
 #include "tma.cuh"
 
@@ -29,10 +35,11 @@ constexpr float KA_P = 8388607.0f;            // 2^23 - 1
 constexpr float KA_MAGIC = 12582912.0f;       // 1.5 * 2^23: a sum that starts at its bits is the float MAGIC + sum (|sum| < 2^22)
 constexpr int KA_MAGIC_BITS = 0x4B400000;
 
-template <int D> struct KaGeom {
-    static constexpr int WARPS = D == 64 ? 8 : D == 128 ? 6 : 3, STAGES = D == 64 ? 3 : 2;
-    static constexpr int TILE = KA_STEP * D, STAGE = 2 * TILE;
-    static constexpr int WARP_BYTES = STAGES * STAGE + STAGES * 32 + 32;   // tiles, scales, barriers
+template <int D, int R> struct KaGeom {
+    // as many as registers (two rows a thread take about 200) and shared memory hold
+    static constexpr int WARPS = D == 256 ? 6 : D == 128 ? (R == 8 ? 12 : 8) : R == 8 ? 16 : 12;
+    static constexpr int TILE = KA_STEP * D;                          // keys, or values, of a step
+    static constexpr int WARP_BYTES = 2 * TILE + 16;                  // and two barriers
     static constexpr int RECORD_ROW = D + 2;
 };
 
@@ -73,7 +80,8 @@ __device__ __forceinline__ float ka_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float ka_sum(int bits) { return __int_as_float(bits) - KA_MAGIC; }
+// two sums that began at MAGIC's bits
+__device__ __forceinline__ uint64_t ka_sum2(int a, int b) { return f2_add(f2(__int_as_float(a), __int_as_float(b)), f2(-KA_MAGIC, -KA_MAGIC)); }
 
 // Steps in front of every sequence, into shared memory, by all threads; returns the steps of the call
 __device__ __forceinline__ long long ka_plan(const KvAttention &a, int R, long long *cum, int2 *info, long long *sums, int threads) {
@@ -142,20 +150,20 @@ struct KaWalk {
 };
 
 template <int D, int R>
-__global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(const __grid_constant__ KvAttention a) {
-    using G = KaGeom<D>;
-    constexpr int NR = R / 8, KS = D / 32, NT = D / 8, STAGES = G::STAGES, THREADS = G::WARPS * 32;
+__global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kernel(const __grid_constant__ KvAttention a) {
+    using G = KaGeom<D, R>;
+    constexpr int NR = R / 8, KS = D / 32, NT = D / 8, THREADS = G::WARPS * 32;
     constexpr int TERMS = R == 8 ? 2 : 3;     // products per tile and 32 of the contraction
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long sums[G::WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    unsigned char *mine = smem + warp * (STAGES * G::STAGE);
-    float *scales = reinterpret_cast<float *>(smem + G::WARPS * STAGES * G::STAGE) + warp * STAGES * 8;
-    const uint32_t bars = smem_u32(smem) + G::WARPS * (STAGES * G::STAGE + STAGES * 32) + warp * 32;
+    const uint32_t ks_at = smem_u32(smem) + warp * (2 * G::TILE), vs_at = ks_at + G::TILE;
+    const uint32_t k_bar = smem_u32(smem) + G::WARPS * (2 * G::TILE) + warp * 16, v_bar = k_bar + 8;
     long long *cum = reinterpret_cast<long long *>(smem + G::WARPS * G::WARP_BYTES);
     int2 *info = reinterpret_cast<int2 *>(cum + a.l.n_seq + 1);
     if (lane == 0) {
-        for (int i = 0; i < STAGES; ++i) mbar_init(bars + i * 8, 1);
+        mbar_init(k_bar, 1);
+        mbar_init(v_bar, 1);
         mbar_fence_init();
     }
     __syncwarp();
@@ -176,58 +184,54 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
     // ---- fetching: lane i < 4 looks after the step's i-th group of 16 keys ----
     KaWalk f;
     f.seek(a, cum, info, R, u0);
-    int ahead = 0, next_id;                   // steps fetched; the page of this lane's group in the next one
+    int next_id = -1, ahead = 0;              // the page of this lane's group in the step that is fetched next; steps fetched
     auto groups_of = [&](const KaWalk &x) { return min(4, (x.s.start + x.s.rows - (x.s.lo + x.step * KA_STEP) + KV_GROUP - 1) / KV_GROUP); };
-    auto page_of = [&](const KaWalk &x) {
-        int id = -1;
-        if (lane < groups_of(x)) {
-            const int at = (x.s.lo + x.step * KA_STEP + KV_GROUP * lane) >> a.l.page_shift;
-            if (at < a.l.max_pages) id = __ldg(a.l.table + (size_t)x.seq * a.l.max_pages + at);
+    auto page = [&]() {
+        next_id = -1;
+        if (lane < groups_of(f)) {
+            const int at = (f.s.lo + f.step * KA_STEP + KV_GROUP * lane) >> a.l.page_shift;
+            if (at < a.l.max_pages) next_id = __ldg(a.l.table + (size_t)f.seq * a.l.max_pages + at);
             if (at >= a.l.max_pages) atomicExch(a.status, YSCV_DEV_POS_OVERFLOW);
-            else if (id < 0 || id >= a.l.n_pages) { id = -1; atomicExch(a.status, YSCV_DEV_BAD_NUMBER); }
+            else if (next_id < 0 || next_id >= a.l.n_pages) { next_id = -1; atomicExch(a.status, YSCV_DEV_BAD_NUMBER); }
         }
-        return id;
     };
     const int piece = min(a.l.page, KA_STEP) / KV_GROUP;   // groups that lie together
-    auto fetch = [&]() {
-        const int st = ahead % STAGES, id = next_id;
-        const uint32_t bar = bars + st * 8, to = smem_u32(mine) + st * G::STAGE;
-        const unsigned there = __ballot_sync(0xffffffffu, id >= 0);
-        if (lane == 0) mbar_expect_tx(bar, __popc(there) * (2 * KV_GROUP * D));
+    size_t from = 0;                          // the lane's bytes in the pool, keys and values alike, and how many it copies
+    int bytes = 0, all_bytes = 0;
+    float next_ks = 0.0f, next_vs = -1.0f;    // scales of the lane's group; values' -1: no such keys
+    auto copy = [&](const int8_t *pool, uint32_t to, uint32_t bar) {
+        if (lane == 0) mbar_expect_tx(bar, all_bytes);
         __syncwarp();
-        if (lane < 4) {
-            const uint32_t sc = smem_u32(scales + st * 8 + lane);
-            if (id >= 0) {
-                const size_t s_at = (size_t)id * a.l.n_kv + f.head;
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(sc), "l"(a.l.ks + s_at) : "memory");
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(sc + 16), "l"(a.l.vs + s_at) : "memory");
-                if (lane % piece == 0) {
-                    const int groups = min(piece, groups_of(f) - lane);
-                    const size_t at = kv_group_at(a.l, id, f.head, ((f.s.lo + f.step * KA_STEP + KV_GROUP * lane) & (a.l.page - 1)) / KV_GROUP);
-                    bulk_load(to + lane * (KV_GROUP * D), a.l.k + at, groups * KV_GROUP * D, bar);
-                    bulk_load(to + G::TILE + lane * (KV_GROUP * D), a.l.v + at, groups * KV_GROUP * D, bar);
-                }
-            } else {
-                scales[st * 8 + lane] = 0.0f;
-                scales[st * 8 + 4 + lane] = -1.0f;       // no such keys
-            }
+        if (bytes > 0) bulk_load(to + lane * (KV_GROUP * D), pool + from, bytes, bar);
+    };
+    auto fetch_keys = [&]() {
+        const bool there = next_id >= 0;
+        all_bytes = __popc(__ballot_sync(0xffffffffu, there)) * (KV_GROUP * D);
+        bytes = 0;
+        next_ks = 0.0f;
+        next_vs = -1.0f;
+        if (there) {
+            const size_t s_at = (size_t)next_id * a.l.n_kv + f.head;
+            next_ks = __ldg(a.l.ks + s_at);
+            next_vs = __ldg(a.l.vs + s_at);
+            from = kv_group_at(a.l, next_id, f.head, ((f.s.lo + f.step * KA_STEP + KV_GROUP * lane) & (a.l.page - 1)) / KV_GROUP);
+            if (lane % piece == 0) bytes = min(piece, groups_of(f) - lane) * (KV_GROUP * D);
         }
-        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        copy(a.l.k, ks_at, k_bar);
         if (++ahead < n) {
             f.next(a, info, R);
-            next_id = page_of(f);
+            page();
         }
     };
-    next_id = page_of(f);
-    for (int i = 0; i < STAGES - 1; ++i) {
-        if (i < n) fetch();
-        else asm volatile("cp.async.commit_group;\n" ::: "memory");
-    }
+    page();
+    fetch_keys();
+    copy(a.l.v, vs_at, v_bar);
 
     KaWalk c;
     c.seek(a, cum, info, R, u0);
     uint32_t qa[KS][NR == 1 ? 6 : 12];        // the query's digits as operands
-    float qs[NR], m[NR], l[NR], o[NT][2 * NR];
+    float qs[NR], m[NR], l[NR];
+    uint64_t o[NT][NR];                       // two columns each
     int lim[NR], low[NR];
     const int first = t < 2 ? 0 : 2;          // of its four tokens of a group, which two a thread has in the first tile
     const uint32_t sel0 = t < 2 ? 0x5410u : 0x1054u, sel1 = t < 2 ? 0x7632u : 0x3276u;
@@ -239,10 +243,8 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
     const uint32_t v_lane = ((lane >> 3) & 1) * (KV_GROUP * D) + ((lane >> 4) * 8 + r8) * 16;
 
     bool begin = true, alive = true;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
-        __syncwarp();                          // every lane is done with the stage that is filled now
-        if (i + STAGES - 1 < n) fetch();
-        else asm volatile("cp.async.commit_group;\n" ::: "memory");
         const int key0 = c.s.lo + c.step * KA_STEP;
         if (begin) {
             begin = false;
@@ -253,21 +255,18 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
                 lim[r] = !live ? 0 : a.causal ? c.s.start + s + 1 : c.s.start + c.s.rows;
                 low[r] = a.window > 0 ? c.s.start + s + 1 - a.window : 0;
                 const float *src = a.q + (size_t)(a.offsets[c.seq] + (live ? s : 0)) * a.q_stride + (size_t)(c.head * a.group + (live ? pair - s * a.group : 0)) * D;
-                float x[KS][8], most = 0.0f, bad = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float *p = src + 32 * k + 16 * h + 4 * t;
-                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (live) y = a.wide ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
-                        x[k][4 * h] = y.x; x[k][4 * h + 1] = y.y; x[k][4 * h + 2] = y.z; x[k][4 * h + 3] = y.w;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        most = fmaxf(most, fabsf(x[k][j]));
-                        bad = fmaf(x[k][j], 0.0f, bad);
-                    }
+                // (read twice, from L1 the second time: kept in registers between the two it would be spilled)
+                auto load = [&](int k, int h) {
+                    const float *p = src + 32 * k + 16 * h + 4 * t;
+                    if (!live) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    return a.wide ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+                };
+                float most = 0.0f, bad = 0.0f;
+#pragma unroll 4
+                for (int k = 0; k < 2 * KS; ++k) {
+                    const float4 y = load(k >> 1, k & 1);
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
+                    bad = fmaf(y.x, 0.0f, fmaf(y.y, 0.0f, fmaf(y.z, 0.0f, fmaf(y.w, 0.0f, bad))));
                 }
 #pragma unroll
                 for (int d = 1; d < 4; d <<= 1) {
@@ -282,10 +281,12 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
                     uint32_t dig[3][2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
+                        const float4 y = load(k, h);
+                        const float x[4] = {y.x, y.y, y.z, y.w};
                         dig[0][h] = dig[1][h] = dig[2][h] = 0u;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int v = __float2int_rn(fminf(fmaxf(x[k][4 * h + j] * up, -KA_Q), KA_Q));
+                            const int v = __float2int_rn(fminf(fmaxf(x[j] * up, -KA_Q), KA_Q));
                             const int d0 = (int)(int8_t)v, v1 = (v - d0) >> 8, d1 = (int)(int8_t)v1, d2 = (v1 - d1) >> 8;
                             dig[0][h] |= (uint32_t)(d0 & 255) << (8 * j);
                             dig[1][h] |= (uint32_t)(d1 & 255) << (8 * j);
@@ -306,16 +307,16 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 2 * NR; ++e) o[j][e] = 0.0f;
+                for (int r = 0; r < NR; ++r) o[j][r] = 0ull;
         }
-        const int st = i % STAGES;
-        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 1) : "memory");
-        alive = mbar_wait(bars + st * 8, (uint32_t)(i / STAGES) & 1u, a.status);
-        alive = __all_sync(0xffffffffu, alive);
+        float kscale[4], vscale[4];
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp) {
+            kscale[grp] = __shfl_sync(0xffffffffu, next_ks, grp);
+            vscale[grp] = __shfl_sync(0xffffffffu, next_vs, grp);
+        }
+        alive = __all_sync(0xffffffffu, mbar_wait(k_bar, (uint32_t)i & 1u, a.status));
         if (!alive) break;
-        const uint32_t ks_at = smem_u32(mine) + st * G::STAGE, vs_at = ks_at + G::TILE;
-        const float4 ksc = *reinterpret_cast<const float4 *>(scales + st * 8), vsc = *reinterpret_cast<const float4 *>(scales + st * 8 + 4);
-        const float kscale[4] = {ksc.x, ksc.y, ksc.z, ksc.w}, vscale[4] = {vsc.x, vsc.y, vsc.z, vsc.w};
         // ---- scores ----
         float s[NR][16];                       // [row][4 group + token of the thread], tile order
 #pragma unroll
@@ -343,15 +344,15 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        const float d2 = ka_sum(acc[tile][0][2 * r + e]);
-                        const float d1 = ka_sum(NR == 1 ? acc[tile][0][2 + e] : acc[tile][1][2 * r + e]);
-                        const float d0 = ka_sum(acc[tile][TERMS - 1][2 * r + e]);
-                        s[r][4 * grp + 2 * tile + e] = fmaf(d2, 65536.0f, fmaf(d1, 256.0f, d0)) * (qs[r] * kscale[grp]);
-                    }
+                for (int r = 0; r < NR; ++r) {
+                    const int *m1 = NR == 1 ? acc[tile][0] + 2 : acc[tile][1] + 2 * r, *m0 = acc[tile][TERMS - 1] + 2 * r, *m2 = acc[tile][0] + 2 * r;
+                    const float f = qs[r] * kscale[grp];
+                    const uint64_t x = f2_fma(ka_sum2(m2[0], m2[1]), f2(65536.0f, 65536.0f), f2_fma(ka_sum2(m1[0], m1[1]), f2(256.0f, 256.0f), ka_sum2(m0[0], m0[1])));
+                    f2_get(f2_mul(x, f2(f, f)), s[r][4 * grp + 2 * tile], s[r][4 * grp + 2 * tile + 1]);
+                }
         }
+        __syncwarp();                          // every lane is done with the keys
+        if (i + 1 < n) fetch_keys();
         bool edge = vscale[0] < 0.0f || vscale[1] < 0.0f || vscale[2] < 0.0f || vscale[3] < 0.0f;
 #pragma unroll
         for (int r = 0; r < NR; ++r) edge |= key0 + KA_STEP > lim[r] || key0 < low[r];
@@ -403,6 +404,8 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
             w0[r] = beta * (vmost > 0.0f ? vmost : 0.0f) * (1.0f / KA_P);
         }
         // ---- weighted values ----
+        alive = __all_sync(0xffffffffu, mbar_wait(v_bar, (uint32_t)i & 1u, a.status));
+        if (!alive) break;
 #pragma unroll
         for (int j = 0; j < NT; j += 2) {
             int acc[2][TERMS][4];
@@ -429,16 +432,16 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float d2 = ka_sum(acc[tile][0][2 * r + e]);
-                        const float d1 = ka_sum(NR == 1 ? acc[tile][0][2 + e] : acc[tile][1][2 * r + e]);
-                        const float d0 = ka_sum(acc[tile][TERMS - 1][2 * r + e]);
-                        float &x = o[j + tile][2 * r + e];
-                        x = fmaf(d2, w0[r] * 65536.0f, fmaf(d1, w0[r] * 256.0f, fmaf(d0, w0[r], x * alpha[r])));
-                    }
+                for (int r = 0; r < NR; ++r) {
+                    const int *m1 = NR == 1 ? acc[tile][0] + 2 : acc[tile][1] + 2 * r, *m0 = acc[tile][TERMS - 1] + 2 * r, *m2 = acc[tile][0] + 2 * r;
+                    uint64_t &x = o[j + tile][r];
+                    x = f2_fma(ka_sum2(m2[0], m2[1]), f2(w0[r] * 65536.0f, w0[r] * 65536.0f),
+                               f2_fma(ka_sum2(m1[0], m1[1]), f2(w0[r] * 256.0f, w0[r] * 256.0f),
+                                      f2_fma(ka_sum2(m0[0], m0[1]), f2(w0[r], w0[r]), f2_mul(x, f2(alpha[r], alpha[r])))));
+                }
         }
+        __syncwarp();
+        if (i + 1 < n) copy(a.l.v, vs_at, v_bar);
         // ---- the end of a segment, or of this warp's part of it ----
         const bool last = c.step + 1 == c.s.steps;
         if (last || i + 1 == n) {
@@ -454,11 +457,13 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
                         float *dst = a.out + (size_t)(a.offsets[c.seq] + sq) * a.out_stride + (size_t)(c.head * a.group + pair - sq * a.group) * D + 2 * t;
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
+                            float2 y;
+                            f2_get(f2_mul(o[j][r], f2(inv, inv)), y.x, y.y);
                             if (a.wide) {
-                                *reinterpret_cast<float2 *>(dst + 8 * j) = make_float2(o[j][2 * r] * inv, o[j][2 * r + 1] * inv);
+                                *reinterpret_cast<float2 *>(dst + 8 * j) = y;
                             } else {
-                                dst[8 * j] = o[j][2 * r] * inv;
-                                dst[8 * j + 1] = o[j][2 * r + 1] * inv;
+                                dst[8 * j] = y.x;
+                                dst[8 * j + 1] = y.y;
                             }
                         }
                     }
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
                     // slot 2 w: the segment began in an earlier warp, 2 w + 1: here
                     float *rec = a.records + ((size_t)(2 * w + (i >= c.step)) * R + 8 * r + g) * G::RECORD_ROW;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) *reinterpret_cast<float2 *>(rec + 8 * j + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+                    for (int j = 0; j < NT; ++j) *reinterpret_cast<uint64_t *>(rec + 8 * j + 2 * t) = o[j][r];
                     if (t == 0) *reinterpret_cast<float2 *>(rec + D) = make_float2(m[r], l[r]);
                 }
             }
@@ -475,71 +480,81 @@ __global__ void __launch_bounds__(KaGeom<D>::WARPS * 32, 1) kv_attention_kernel(
         if (i + 1 < n) c.next(a, info, R);
     }
     if (!alive) {   // no copy may be in flight when the CTA leaves (bounded)
-        for (int j = max(0, ahead - STAGES); j < ahead; ++j) mbar_wait(bars + (j % STAGES) * 8, (uint32_t)(j / STAGES) & 1u, nullptr);
+        mbar_wait(k_bar, (uint32_t)(ahead - 1) & 1u, nullptr);
+        mbar_wait(v_bar, (uint32_t)(ahead - 1) & 1u, nullptr);
+        mbar_wait(v_bar, (uint32_t)ahead & 1u, nullptr);
     }
-    asm volatile("cp.async.wait_all;\n" ::: "memory");
 }
 
-// Adds the records of a segment that several warps shared: a CTA per (sequence, KV head) and pair
-template <int D, int R>
-__global__ void __launch_bounds__(128) kv_attention_merge_kernel(const __grid_constant__ KvAttention a) {
+// Adds the records of a segment that several warps shared: a CTA per (sequence, KV head) and pair, a share of the records for each of
+// its W warps: 16 where there are fewer CTAs than four an SM, else 4 (few records each).
+template <int D, int R, int W>
+__global__ void __launch_bounds__(32 * W) kv_attention_merge_kernel(const __grid_constant__ KvAttention a) {
     pdl_wait();
     pdl_trigger();
-    constexpr int ROW = D + 2, PER = 128;
-    __shared__ float wt[PER], red[8];
+    constexpr int ROW = D + 2, C = D / 32;       // columns of a lane, as pairs: 2 lane + 64 e
+    __shared__ __align__(8) float part[W][D];
+    __shared__ float red[W][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seq = blockIdx.x, head = blockIdx.y;
+    const long long share = a.plan[1], base = a.plan[2 + seq];
     const int row0 = a.offsets[seq];
     const KaSeq s = ka_seq(a, a.start[seq], a.offsets[seq + 1] - row0, R);
     if (s.steps == 0) return;
-    const long long share = a.plan[1], base = a.plan[2 + seq];
     for (int pair = blockIdx.z; pair < s.rows * a.group; pair += gridDim.z) {
         const int block = pair / R, r = pair - block * R;
         const long long from = base + ((long long)head * s.blocks + block) * s.steps, to = from + s.steps;
         const long long wa = from / share, wb = (to - 1) / share;
-        if (wa == wb) continue;                // one warp had it all and wrote it
+        if (wa == wb) continue;                  // one warp had it all and wrote it
         const int parts = (int)(wb - wa) + 1;
         auto record = [&](int p) { return a.records + ((size_t)(2 * (wa + p) + (p == 0)) * R + r) * ROW; };
-        float mx = -INFINITY;
-        for (int p = tid; p < parts; p += 128) mx = fmaxf(mx, record(p)[D]);
+        // every warp its records, 32 at a time, by its own maximum
+        float m = -INFINITY, l = 0.0f, acc[C] = {};
+        for (int p0 = warp; p0 < parts; p0 += 32 * W) {
+            const int mine = p0 + W * lane, np = min(32, (parts - p0 + W - 1) / W);
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (mine < parts) ml = *reinterpret_cast<const float2 *>(record(mine) + D);
+            float mx = ml.x;
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        if (lane == 0) red[warp] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        float sum = 0.0f, acc[D / 64] = {};
-        // D values by 128 threads: two threads a value at 64, each half of the records; two values a thread at 256
-        const int col = D == 64 ? tid & 63 : tid, odd = D == 64 ? tid >> 6 : 0, stride = D == 64 ? 2 : 1;
-        for (int p0 = 0; p0 < parts; p0 += PER) {
-            const int np = min(PER, parts - p0);
-            if (tid < np) {
-                const float2 ml = *reinterpret_cast<const float2 *>(record(p0 + tid) + D);
-                const float x = ka_exp2(ml.x - ref);
-                wt[tid] = x;
-                sum = fmaf(x, ml.y, sum);
-            }
-            __syncthreads();
+            for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float old = ka_exp2(m - ref), w = ka_exp2(ml.x - ref);
+            m = m_new;
+            l = fmaf(l, old, w * ml.y);          // (of the lane's records)
+#pragma unroll
+            for (int e = 0; e < C; ++e) acc[e] *= old;
 #pragma unroll 8
-            for (int p = odd; p < np; p += stride) {
-                const float *rec = record(p0 + p);
+            for (int p = 0; p < np; ++p) {
+                const float y = __shfl_sync(0xffffffffu, w, p);
+                const float *rec = record(p0 + W * p) + 2 * lane;
 #pragma unroll
-                for (int e = 0; e < (D == 256 ? 2 : 1); ++e) acc[e] = fmaf(wt[p], rec[col + 128 * e], acc[e]);
+                for (int e = 0; e < C / 2; ++e) {
+                    const float2 v = *reinterpret_cast<const float2 *>(rec + 64 * e);
+                    acc[2 * e] = fmaf(y, v.x, acc[2 * e]);
+                    acc[2 * e + 1] = fmaf(y, v.y, acc[2 * e + 1]);
+                }
             }
-            __syncthreads();
         }
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) red[4 + warp] = sum;
-        if (odd) wt[col] = acc[0];
+        for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+        for (int e = 0; e < C / 2; ++e) *reinterpret_cast<float2 *>(&part[warp][2 * lane + 64 * e]) = make_float2(acc[2 * e], acc[2 * e + 1]);
+        if (lane == 0) { red[warp][0] = m; red[warp][1] = l; }
         __syncthreads();
-        sum = (red[4] + red[5]) + (red[6] + red[7]);
+        float all = red[0][0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) all = fmaxf(all, red[i][0]);
+        const float ref = all == -INFINITY ? 0.0f : all;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) sum = fmaf(ka_exp2(red[i][0] - ref), red[i][1], sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int sq = pair / a.group;
         float *dst = a.out + (size_t)(row0 + sq) * a.out_stride + (size_t)(head * a.group + pair - sq * a.group) * D;
-        if (!odd) {
-            if (D == 64) acc[0] += wt[col];
+        for (int c = tid; c < D; c += 32 * W) {
+            float x = 0.0f;
 #pragma unroll
-            for (int e = 0; e < (D == 256 ? 2 : 1); ++e) dst[col + 128 * e] = acc[e] * inv;
+            for (int i = 0; i < W; ++i) x = fmaf(ka_exp2(red[i][0] - ref), part[i][c], x);
+            dst[c] = x * inv;
         }
         __syncthreads();
     }
@@ -548,24 +563,35 @@ __global__ void __launch_bounds__(128) kv_attention_merge_kernel(const __grid_co
 // ---- host -----------------------------------------------------------------------------------------
 static int ka_rows(size_t d, size_t pairs) { return d == 256 || pairs <= 8 ? 8 : 16; }
 
-static size_t ka_smem(size_t d, size_t n_seq) {
-    const size_t per = d == 64 ? KaGeom<64>::WARPS * KaGeom<64>::WARP_BYTES : d == 128 ? KaGeom<128>::WARPS * KaGeom<128>::WARP_BYTES
-                                                                                     : KaGeom<256>::WARPS * KaGeom<256>::WARP_BYTES;
-    return per + (n_seq + 1) * sizeof(long long) + n_seq * sizeof(int2);
+// warps of a CTA, and bytes of one's buffers
+static void ka_geometry(size_t d, int R, size_t &warps, size_t &bytes) {
+    auto of = [&](auto g) { warps = decltype(g)::WARPS; bytes = decltype(g)::WARP_BYTES; };
+    if (d == 64) R == 8 ? of(KaGeom<64, 8>()) : of(KaGeom<64, 16>());
+    else if (d == 128) R == 8 ? of(KaGeom<128, 8>()) : of(KaGeom<128, 16>());
+    else of(KaGeom<256, 8>());
+}
+static size_t ka_smem(size_t d, int R, size_t n_seq) {
+    size_t warps, bytes;
+    ka_geometry(d, R, warps, bytes);
+    return warps * bytes + (n_seq + 1) * sizeof(long long) + n_seq * sizeof(int2);
 }
 static size_t ka_plan_bytes(size_t n_seq) { return (2 + n_seq + 1) * sizeof(long long) + 15 & ~(size_t)15; }
 static size_t ka_bytes(const yscv_cuda_ctx *ctx, size_t d, size_t n_seq, int R) {
-    const size_t warps = (size_t)ctx->sm_count * (d == 64 ? KaGeom<64>::WARPS : d == 128 ? KaGeom<128>::WARPS : KaGeom<256>::WARPS);
+    size_t warps, bytes;
+    ka_geometry(d, R, warps, bytes);
+    warps *= ctx->sm_count;
     return ka_plan_bytes(n_seq) + 2 * warps * R * (d + 2) * sizeof(float);
 }
 
 template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttention &a, size_t pairs) {
     auto kern = kv_attention_kernel<D, R>;
     if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kern), ctx->device, 226 * 1024)) return rc;
-    YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KaGeom<D>::WARPS * 32), ka_smem(D, a.l.n_seq), ctx->stream, a));
+    YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KaGeom<D, R>::WARPS * 32), ka_smem(D, R, a.l.n_seq), ctx->stream, a));
     ctx->launches++;
     const unsigned z = (unsigned)(pairs < 1024 ? pairs : 1024);
-    YSCV_CUDA_TRY(launch_pdl(kv_attention_merge_kernel<D, R>, dim3((unsigned)a.l.n_seq, (unsigned)a.l.n_kv, z), dim3(128), 0, ctx->stream, a));
+    const bool few = (size_t)a.l.n_seq * a.l.n_kv * z < (size_t)4 * ctx->sm_count;
+    YSCV_CUDA_TRY(launch_pdl(few ? kv_attention_merge_kernel<D, R, 16> : kv_attention_merge_kernel<D, R, 4>,
+                             dim3((unsigned)a.l.n_seq, (unsigned)a.l.n_kv, z), dim3(few ? 512 : 128), 0, ctx->stream, a));
     ctx->launches++;
     YSCV_CUDA_TRY(cudaGetLastError());
     ctx->last_kernel = "kv_block_attention(steps,imma)";
@@ -584,9 +610,9 @@ static int ka_check(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_
         return fail(YSCV_CUDA_ERR_UNSUPPORTED, "attention takes heads of 64, 128 or 256, got %zu", pool->d_head);
     if (n_q == 0 || n_q % pool->n_kv != 0) return fail(YSCV_CUDA_ERR_BAD_ARG, "n_q=%zu must be a positive multiple of n_kv=%zu", n_q, pool->n_kv);
     if (n_q > 65535 || rows * n_q >= (1u << 31) || most_rows * n_q >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows or heads");
-    if (ka_smem(pool->d_head, pool->n_seq) > 226 * 1024)
+    if (ka_smem(pool->d_head, 8, pool->n_seq) > 226 * 1024 || ka_smem(pool->d_head, 16, pool->n_seq) > 226 * 1024)
         return fail(YSCV_CUDA_ERR_UNSUPPORTED, "attention takes pools of up to %zu sequences at this head size",
-                    (226 * 1024 - ka_smem(pool->d_head, 0)) / (sizeof(long long) + sizeof(int2)));
+                    (226 * 1024 - std::max(ka_smem(pool->d_head, 8, 0), ka_smem(pool->d_head, 16, 0))) / (sizeof(long long) + sizeof(int2)));
     return YSCV_CUDA_OK;
 }
 
