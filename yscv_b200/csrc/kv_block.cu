@@ -2,12 +2,14 @@
 //
 // A block of the cache is a page's tokens of one KV head, keys or values; its scale s = fp32(m / 127), m its largest magnitude,
 // its values rne(x / s) of the real quotient. The quotient is taken as x * (1 / s) in fp32, which is within 2^-15 of it (three
-// roundings of 2^-24 on at most 127.5); where that lies within 2^-13 of a border between two whole numbers the fp64
-// quotient decides. That one is exact enough: x and s have 24 bits, so x / s is a border or 2^-26 of its size away from it.
+// roundings of 2^-24 on at most 127.5); where that lies within 2^-13 of a border b between two whole numbers, x - b s decides, whose
+// sign one fused multiply-add has exactly.
 //
 // Append: one CTA per (page that a sequence's rows touch, head, keys or values), so nobody else writes the block or its scale.
-// Bound: bytes (4 in, 1 out per value), a decode step: latency, three dependent loads deep. Values leave as whole 16-byte
-// rows of 16 tokens, turned in shared memory; the first and last group, which may hold other tokens, byte by byte.
+// Bound: bytes (4 in, 1 out per value), a decode step: latency, three dependent loads deep. Numbers go through shared memory
+// and leave as the cache has them, lanes side by side: 16 bytes of a token's keys, 16 tokens of a value row (a group that other tokens
+// share: byte by byte). 3700 rows of 8 heads of 128, pages of 32: 33.9 us with keys stored 4 bytes and value rows gathered a
+// byte at a time and an index division per access, APPEND so.
 #include <cfloat>
 
 #include "kv_pool.cuh"
@@ -19,11 +21,21 @@ struct KvRows {
     size_t stride;                 // floats between rows
 };
 
+// The whole number next to the border b on the side that the sign of `off` says, the even one on the border itself
+__device__ __forceinline__ float kv_side(float b, float off) {
+    const float below = b - 0.5f;
+    return off > 0.0f || (off == 0.0f && ((int)below & 1)) ? below + 1.0f : below;
+}
+__device__ __forceinline__ bool kv_near_border(float v, float r) { return fabsf(fabsf(v - r) - 0.5f) < 1.220703125e-4f; }
+
 // Whole number nearest to x / s. NaN: 0, infinities: +-127.
 __device__ __forceinline__ int kv_quantise(float x, float s, float inv) {
     const float v = x * inv;
     float r = rintf(v);
-    if (fabsf(fabsf(v - r) - 0.5f) < 1.220703125e-4f) r = (float)rint((double)x / (double)s);
+    if (kv_near_border(v, r)) {
+        const float b = floorf(v) + 0.5f;
+        r = kv_side(b, fmaf(-b, s, x));
+    }
     r = fminf(fmaxf(r, -127.0f), 127.0f);
     return x == x ? (int)r : 0;
 }
@@ -44,7 +56,11 @@ __device__ __forceinline__ uint32_t kv_requantise(uint32_t w, int count, float r
         const int q = (int)(int8_t)(w >> (8 * i));
         const float v = (float)q * ratio;
         float r = rintf(v);
-        if (fabsf(fabsf(v - r) - 0.5f) < 1.220703125e-4f) r = (float)rint((double)q * (double)s_old / (double)s_new);
+        if (kv_near_border(v, r)) {
+            // q s_old - b s_new: the product's rounding apart, the difference of what is left is exact so near the border
+            const float b = floorf(v) + 0.5f, p = (float)q * s_old;
+            r = kv_side(b, fmaf(-b, s_new, p) + fmaf((float)q, s_old, -p));
+        }
         out = (out & ~(255u << (8 * i))) | (uint32_t)((int)r & 255) << (8 * i);
     }
     return out;
@@ -65,11 +81,22 @@ __device__ __forceinline__ KvSpan kv_span(const KvRows &r, int seq) {
 }
 
 constexpr int KVB_KEEP = 8;        // float4 a thread keeps in registers between the maximum and the quantising
+__host__ __device__ constexpr int kv_stage_pitch(int d) { return d + 16; }   // bytes of a staged token
+
+// four tokens' words of four d -> four d's words of four tokens
+__device__ __forceinline__ void kv_turn(const uint32_t (&w)[4], uint32_t (&out)[4]) {
+    const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);   // {0.0, 1.0, 0.1, 1.1}, ...
+    const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);   // {0.2, 1.2, 0.3, 1.3}, ...
+    out[0] = __byte_perm(a, b, 0x5410);
+    out[1] = __byte_perm(a, b, 0x7632);
+    out[2] = __byte_perm(c, d, 0x5410);
+    out[3] = __byte_perm(c, d, 0x7632);
+}
 
 template <int T>
-__global__ void __launch_bounds__(T) kv_append_kernel(const KvLayer l, const float *__restrict__ k, const float *__restrict__ v, const KvRows rows,
+__global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l, const float *__restrict__ k, const float *__restrict__ v, const KvRows rows,
                                                       int per_seq, int wide, int *__restrict__ status) {
-    extern __shared__ __align__(16) unsigned char stage[];   // values: [tokens][d + 4]
+    extern __shared__ __align__(16) unsigned char stage[];   // [tokens][kv_stage_pitch(d)]
     __shared__ float red[T / 32];
     pdl_wait();
     pdl_trigger();
@@ -78,38 +105,39 @@ __global__ void __launch_bounds__(T) kv_append_kernel(const KvLayer l, const flo
     const KvSpan sp = kv_span(rows, seq);
     if (!sp.live) return;
     const long long end = (long long)sp.p0 + sp.rows;
-    const int d4 = l.d >> 2;
-    const float *src = (values ? v : k) + (size_t)sp.row0 * rows.stride + (size_t)head * l.d;
+    // a thread has four d of every `step`-th token
+    const int d4 = l.d >> 2, step = T / d4, c = tid % d4, first = tid / d4 < step ? tid / d4 : 1 << 30, pitch = kv_stage_pitch(l.d);
+    const float *src = (values ? v : k) + (size_t)sp.row0 * rows.stride + (size_t)head * l.d + 4 * c;
     for (long long pg = (sp.p0 >> l.page_shift) + blockIdx.x % per_seq; (pg << l.page_shift) < end; pg += per_seq) {
         if (pg >= l.max_pages) {
             if (tid == 0) atomicExch(status, YSCV_DEV_POS_OVERFLOW);
             return;
         }
         const int id = l.table[(size_t)seq * l.max_pages + pg];
-        if (id < 0 || id >= l.n_pages) {
-            if (tid == 0) atomicExch(status, YSCV_DEV_BAD_NUMBER);
-            continue;
-        }
         const long long base = pg << l.page_shift;
         const int t0 = (int)max(0ll, (long long)sp.p0 - base), t1 = (int)min((long long)l.page, end - base);   // new tokens of the page
-        const int row = (int)(base + t0 - sp.p0), items = (t1 - t0) * d4;
-        float *scale = (values ? l.vs : l.ks) + (size_t)id * l.n_kv + head;
-        const float s_old = t0 > 0 ? *scale : 0.0f;
+        const int n = t1 - t0;
+        const float *row = src + (size_t)(base + t0 - sp.p0) * rows.stride;
         // largest magnitude of the new tokens
         float4 x[KVB_KEEP];
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < KVB_KEEP; ++i) {
-            const int at = tid + T * i;
-            if (at < items) {
-                const int t = at / d4, c = at - t * d4;
-                x[i] = kv_load4(src + (size_t)(row + t) * rows.stride + 4 * c, wide);
-                m = fmaxf(m, fmaxf(fmaxf(kv_magnitude(x[i].x), kv_magnitude(x[i].y)), fmaxf(kv_magnitude(x[i].z), kv_magnitude(x[i].w))));
-            }
+            const int t = first + step * i;
+            if (t < n) x[i] = kv_load4(row + (size_t)t * rows.stride, wide);
         }
-        for (int at = tid + T * KVB_KEEP; at < items; at += T) {
-            const int t = at / d4, c = at - t * d4;
-            const float4 y = kv_load4(src + (size_t)(row + t) * rows.stride + 4 * c, wide);
+        if (id < 0 || id >= l.n_pages) {
+            if (tid == 0) atomicExch(status, YSCV_DEV_BAD_NUMBER);
+            continue;
+        }
+        float *scale = (values ? l.vs : l.ks) + (size_t)id * l.n_kv + head;
+        const float s_old = t0 > 0 ? *scale : 0.0f;
+#pragma unroll
+        for (int i = 0; i < KVB_KEEP; ++i)
+            if (first + step * i < n)
+                m = fmaxf(m, fmaxf(fmaxf(kv_magnitude(x[i].x), kv_magnitude(x[i].y)), fmaxf(kv_magnitude(x[i].z), kv_magnitude(x[i].w))));
+        for (int t = first + step * KVB_KEEP; t < n; t += step) {
+            const float4 y = kv_load4(row + (size_t)t * rows.stride, wide);
             m = fmaxf(m, fmaxf(fmaxf(kv_magnitude(y.x), kv_magnitude(y.y)), fmaxf(kv_magnitude(y.z), kv_magnitude(y.w))));
         }
 #pragma unroll
@@ -139,40 +167,49 @@ __global__ void __launch_bounds__(T) kv_append_kernel(const KvLayer l, const flo
                 w.w = kv_requantise(w.w, count - 12, ratio, s_old, s);
                 *p = w;
             }
-            if (values) __syncthreads();   // (the last row's bytes of new tokens follow below)
         }
         if (tid == 0 && (t0 == 0 || grows)) *scale = s;
-        auto put = [&](int at, const float4 &y) {
-            const int t = at / d4, c = at - t * d4;
-            const uint32_t w = (uint32_t)(kv_quantise(y.x, s, inv) & 255) | (uint32_t)(kv_quantise(y.y, s, inv) & 255) << 8 |
-                               (uint32_t)(kv_quantise(y.z, s, inv) & 255) << 16 | (uint32_t)(kv_quantise(y.w, s, inv) & 255) << 24;
-            if (values) {
-                *reinterpret_cast<uint32_t *>(stage + t * (l.d + 4) + 4 * c) = w;
-            } else {
-                const int token = t0 + t;
-                *reinterpret_cast<uint32_t *>(page + (token / KV_GROUP) * (KV_GROUP * l.d) + (c >> 2) * 256 + (token % KV_GROUP) * 16 + (c & 3) * 4) = w;
-            }
+        auto put = [&](int t, const float4 &y) {
+            *reinterpret_cast<uint32_t *>(stage + t * pitch + 4 * c) =
+                (uint32_t)(kv_quantise(y.x, s, inv) & 255) | (uint32_t)(kv_quantise(y.y, s, inv) & 255) << 8 |
+                (uint32_t)(kv_quantise(y.z, s, inv) & 255) << 16 | (uint32_t)(kv_quantise(y.w, s, inv) & 255) << 24;
         };
 #pragma unroll
         for (int i = 0; i < KVB_KEEP; ++i)
-            if (tid + T * i < items) put(tid + T * i, x[i]);
-        for (int at = tid + T * KVB_KEEP; at < items; at += T) {
-            const int t = at / d4, c = at - t * d4;
-            put(at, kv_load4(src + (size_t)(row + t) * rows.stride + 4 * c, wide));
-        }
-        if (values) {
-            __syncthreads();
-            const int g0 = t0 / KV_GROUP, g1 = (t1 + KV_GROUP - 1) / KV_GROUP;
-            for (int i = tid; i < (g1 - g0) * l.d; i += T) {
-                const int g = g0 + i / l.d, c = i % l.d, a = g * KV_GROUP - t0;
-                int8_t *p = page + ((size_t)g * l.d + c) * KV_GROUP;
-                if (a >= 0 && g * KV_GROUP + KV_GROUP <= t1) {
-                    uint32_t w[4] = {0u, 0u, 0u, 0u};
+            if (first + step * i < n) put(first + step * i, x[i]);
+        for (int t = first + step * KVB_KEEP; t < n; t += step) put(t, kv_load4(row + (size_t)t * rows.stride, wide));
+        __syncthreads();   // (the last value row's bytes of new tokens follow those that were rounded again)
+        if (!values) {
+            const int i1 = ((t1 + KV_GROUP - 1) / KV_GROUP) * l.d;
+            for (int i = t0 / KV_GROUP * l.d + tid; i < i1; i += T) {
+                const int g = i / l.d, in = i - g * l.d, t = g * KV_GROUP + in % KV_GROUP - t0;
+                if (t >= 0 && t < n) reinterpret_cast<uint4 *>(page)[i] = *reinterpret_cast<const uint4 *>(stage + t * pitch + (in / KV_GROUP) * 16);
+            }
+        } else {
+            const int i1 = ((t1 + KV_GROUP - 1) / KV_GROUP) * d4;
+            for (int i = t0 / KV_GROUP * d4 + tid; i < i1; i += T) {
+                const int g = i / d4, at = i - g * d4, t = g * KV_GROUP - t0;     // four rows of the group's d
+                int8_t *p = page + (size_t)i * (4 * KV_GROUP);
+                const unsigned char *from = stage + t * pitch + 4 * at;
+                if (t >= 0 && t + KV_GROUP <= n) {
+                    uint32_t out[4][4];
 #pragma unroll
-                    for (int j = 0; j < KV_GROUP; ++j) w[j >> 2] |= (uint32_t)stage[(a + j) * (l.d + 4) + c] << (8 * (j & 3));
-                    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t w[4], r[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t *>(from + (4 * q + j) * pitch);
+                        kv_turn(w, r);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) out[j][q] = r[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) reinterpret_cast<uint4 *>(p)[j] = make_uint4(out[j][0], out[j][1], out[j][2], out[j][3]);
                 } else {
-                    for (int j = max(0, -a); j < min(KV_GROUP, t1 - g * KV_GROUP); ++j) p[j] = (int8_t)stage[(a + j) * (l.d + 4) + c];
+                    for (int q = max(0, -t); q < min(KV_GROUP, n - t); ++q) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t *>(from + q * pitch);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) p[j * KV_GROUP + q] = (int8_t)(w >> (8 * j));
+                    }
                 }
             }
         }
@@ -180,13 +217,13 @@ __global__ void __launch_bounds__(T) kv_append_kernel(const KvLayer l, const flo
     }
 }
 
-// Cached rows as f32: a CTA per (page, head, keys or values). A thread takes 16 bytes, 16 values of a token's keys or one value
-// of 16 tokens.
-__global__ void __launch_bounds__(128) kv_read_kernel(const KvLayer l, const KvRows rows, int per_seq, float *__restrict__ k_out, float *__restrict__ v_out,
-                                                      int *__restrict__ status) {
+// Cached rows as f32: a CTA per (page, head, keys or values), a warp per group of 16 tokens. Keys: a lane has four d of a token, so
+// that a row leaves in whole lines; values: one d of 16 tokens.
+__global__ void __launch_bounds__(128, 8) kv_read_kernel(const KvLayer l, const KvRows rows, int per_seq, float *__restrict__ k_out, float *__restrict__ v_out,
+                                                      int wide, int *__restrict__ status) {
     pdl_wait();
     pdl_trigger();
-    const int tid = threadIdx.x, seq = blockIdx.x / per_seq, head = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, seq = blockIdx.x / per_seq, head = blockIdx.y;
     const bool values = blockIdx.z != 0;
     const KvSpan sp = kv_span(rows, seq);
     if (!sp.live) return;
@@ -205,25 +242,37 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const KvLayer l, const KvR
         const long long base = pg << l.page_shift;
         const int t0 = (int)max(0ll, (long long)sp.p0 - base), t1 = (int)min((long long)l.page, end - base);
         const float s = (values ? l.vs : l.ks)[(size_t)id * l.n_kv + head];
-        const int g0 = t0 / KV_GROUP, g1 = (t1 + KV_GROUP - 1) / KV_GROUP;
-        const uint4 *page = reinterpret_cast<const uint4 *>((values ? l.v : l.k) + kv_group_at(l, id, head, 0));
+        const int8_t *page = (values ? l.v : l.k) + kv_group_at(l, id, head, 0);
         float *out = dst + (base - sp.p0) * (long long)rows.stride;    // the row of the page's first token
-        for (int i = g0 * l.d + tid; i < g1 * l.d; i += 128) {
-            const int g = i / l.d, in = i - g * l.d;
-            const uint4 w = page[i];
-            const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+        for (int g = t0 / KV_GROUP + (tid >> 5); g * KV_GROUP < t1; g += 4) {
+            const int a = max(t0, g * KV_GROUP), b = min(t1, g * KV_GROUP + KV_GROUP);
+            const int8_t *group = page + (size_t)g * (KV_GROUP * l.d);
+            float *o = out + (size_t)a * rows.stride;
             if (values) {
+                for (int c = lane; c < l.d; c += 32) {
+                    const uint4 w = reinterpret_cast<const uint4 *>(group)[c];
+                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int j = 0; j < KV_GROUP; ++j) {
-                    const int t = g * KV_GROUP + j;
-                    if (t >= t0 && t < t1) out[(size_t)t * rows.stride + in] = (float)(int8_t)(word[j >> 2] >> (8 * (j & 3))) * s;
+                    for (int j = 0; j < KV_GROUP; ++j) {
+                        const int t = g * KV_GROUP + j;
+                        if (t >= a && t < b) o[(size_t)(t - a) * rows.stride + c] = (float)(int8_t)(word[j >> 2] >> (8 * (j & 3))) * s;
+                    }
                 }
             } else {
-                const int t = g * KV_GROUP + in % KV_GROUP;
-                if (t < t0 || t >= t1) continue;
-                float *o = out + (size_t)t * rows.stride + (in / KV_GROUP) * 16;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = (float)(int8_t)(word[j >> 2] >> (8 * (j & 3))) * s;
+                for (int c = lane; c < l.d >> 2; c += 32) {
+                    const int8_t *from = group + (c >> 2) * 256 + (c & 3) * 4 + (a - g * KV_GROUP) * 16;
+#pragma unroll 8
+                    for (int t = 0; t < b - a; ++t) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t *>(from + t * 16);
+                        const float4 y = make_float4((float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s, (float)(int8_t)(w >> 24) * s);
+                        float *p = o + (size_t)t * rows.stride + 4 * c;
+                        if (wide) {
+                            *reinterpret_cast<float4 *>(p) = y;
+                        } else {
+                            p[0] = y.x; p[1] = y.y; p[2] = y.z; p[3] = y.w;
+                        }
+                    }
+                }
             }
         }
     }
@@ -260,14 +309,15 @@ int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const int per = pages_per_seq(l, most_rows);
     const bool wide = ((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) == 0 && row_stride % 4 == 0;
-    // two warps where a page gets a token or a few, eight for prompts
-    const bool small = most_rows * (size_t)l.d <= 2 * 64 * 4;
+    // threads by what a page gets, so that KVB_KEEP loads a thread hold it: two warps for a token or a few, up to 16
+    const size_t most = (most_rows < pool->page ? most_rows : pool->page) * pool->d_head;
+    const int threads = most <= 2 * 64 * 4 ? 64 : most <= 128 * 4 * KVB_KEEP ? 128 : most <= 256 * 4 * KVB_KEEP ? 256 : 512;
     const dim3 grid((unsigned)(l.n_seq * per), (unsigned)l.n_kv, 2);
     const KvRows rows = {d_offsets, d_start, row_stride};
     // (room for a whole page: a sequence may have more rows than were expected)
-    const size_t smem = (size_t)l.page * (l.d + 4);
-    auto kern = small ? kv_append_kernel<64> : kv_append_kernel<256>;
-    YSCV_CUDA_TRY(launch_pdl(kern, grid, dim3(small ? 64 : 256), smem, ctx->stream, l, d_k, d_v, rows, per, (int)wide, ctx->d_status));
+    const size_t smem = (size_t)l.page * kv_stage_pitch(l.d);
+    auto kern = threads == 64 ? kv_append_kernel<64> : threads == 128 ? kv_append_kernel<128> : threads == 256 ? kv_append_kernel<256> : kv_append_kernel<512>;
+    YSCV_CUDA_TRY(launch_pdl(kern, grid, dim3((unsigned)threads), smem, ctx->stream, l, d_k, d_v, rows, per, (int)wide, ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
     ctx->launches++;
     ctx->last_kernel = "kv_block_append";
@@ -283,7 +333,8 @@ int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
     const int per = pages_per_seq(l, most_rows);
     const KvRows rows = {d_offsets, d_start, row_stride};
     YSCV_CUDA_TRY(launch_pdl(kv_read_kernel, dim3((unsigned)(l.n_seq * per), (unsigned)l.n_kv, 2), dim3(128), 0, ctx->stream, l, rows, per, d_k_out,
-                             d_v_out, ctx->d_status));
+                             d_v_out, (int)(((reinterpret_cast<uintptr_t>(d_k_out) | reinterpret_cast<uintptr_t>(d_v_out)) & 15) == 0 && row_stride % 4 == 0),
+                             ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
     ctx->launches++;
     ctx->last_kernel = "kv_block_read";
