@@ -662,7 +662,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     a.plan = static_cast<long long *>(d_workspace);
     a.records = reinterpret_cast<float *>(static_cast<unsigned char *>(d_workspace) + ka_plan_bytes(pool->n_seq));
     a.status = ctx->d_status;
-    if (kv_prompt_takes(pool->d_head, pool->n_seq, group, most_rows)) return kv_prompt(ctx, a, d_workspace);
+    if (kv_prompt_takes(pool->d_head, pool->n_seq, group, most_rows)) return kv_prompt(ctx, a, d_workspace, rows);
     switch (pool->d_head) {
         case 64: return R == 8 ? ka_launch<64, 8>(ctx, a, pairs) : ka_launch<64, 16>(ctx, a, pairs);
         case 128: return R == 8 ? ka_launch<128, 8>(ctx, a, pairs) : ka_launch<128, 16>(ctx, a, pairs);

@@ -8,22 +8,27 @@
 // A CTA works on tiles of 128 (position, query head) pairs of one KV head and 128 keys:
 //   warp 0       TMEM; the products S = Q K^T and O = P V, both with the A operand in TMEM (from shared memory a product of 128 x 128
 //                reads two operands and takes 125 cycles, with A in TMEM 70): S of the next tile runs under the softmax of this one
-//   warp 1       queries of the next segment into shared memory, by bulk copies
+//   warp 1       queries of the next segment into shared memory, by tensor copies
 //   warps 2, 3   keys and values of the tiles as they are cached, by bulk copies a tile ahead, and what the others have to know
 //   warps 4-7    the tile's bytes as fp16 operands
-//   warps 8-15   softmax, two threads a row: the queries' two terms to TMEM for a segment's first tile; scores from TMEM, the tile's own
-//                maximum and sum, weights back to where the scores were. They keep nothing from tile to tile
+//   warps 8-15   softmax, a thread a row, two tiles at a time: the queries' two terms to TMEM for a segment's first tile; scores from
+//                TMEM, the tile's own maximum and sum, weights back to where the scores were. They keep nothing from tile to tile
 //   warps 16-19  the output in registers, a thread per row: o = o 2^(M - M') + O 2^(m - M'), and results
 // With the output in the softmax threads' registers those have too few left to keep several exponentials in flight: 2048 x 2048
-// keys, 64 / 8 heads of 128, 507 us, a tile of 128 rows 6300 cycles.
+// keys, 64 / 8 heads of 128, 507 us, a tile of 128 rows 6300 cycles. With all eight softmax warps on one tile, which then hand its
+// maxima to each other, a tile takes 3950 cycles, with four warps on each of two tiles 3600.
 // Registers are moved between the warpgroups: 640 threads x 96 = 128 x (56 + 72 + 96 + 96 + 160).
 //
 // Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, with room for KP_BEGIN tiles in front of each
 // segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
 // kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and causal prompts, whose first
-// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 456 us with tiles alone, 210 so; 276 with one, 212 with four).
-// Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128.
+// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 174 us; an earlier form with longer beginnings took
+// 456 us with tiles alone and 210 with room for two).
+// Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128; what holds a tile for 3600
+// is the chain of its two products and its softmax, with as many tiles on their way as TMEM has room for (two), and the issue slots,
+// of which a tile takes 2100 of each scheduler.
 #include <cfloat>
+#include <climits>
 
 #include "attention_tc.cuh"
 #include "kv_attention.cuh"
@@ -31,20 +36,19 @@
 
 namespace yscv {
 
-constexpr int KP_KEYS = 128, KP_ROWS = 128, KP_THREADS = 640, KP_NOTES = 8, KP_BEGIN = 2;
+constexpr int KP_KEYS = 128, KP_ROWS = 128, KP_THREADS = 640, KP_NOTES = 8, KP_BEGIN = 1;
 
 template <int D> struct KpGeom {
     static constexpr int OPERAND = KP_KEYS * D * 2, RAW = KP_KEYS * D;   // keys, or values, of a tile, in fp16 and as cached
-    static constexpr int K_AT = 0, V_AT = 2 * OPERAND;         // two stages of keys, one of values
+    static constexpr int K_AT = 0, V_AT = OPERAND;             // one stage of keys, two of values
     static constexpr int RAW_K = 3 * OPERAND, RAW_V = RAW_K + RAW;
-    static constexpr int Q_AT = RAW_V + RAW;                   // the next segment's queries, f32
-    static constexpr int Q_PITCH = D * 4 + 16;
-    static constexpr int OUT_AT = Q_AT + KP_ROWS * Q_PITCH;    // 4 KB a warp of the output
-    static constexpr int STATS = OUT_AT + 16384;               // [2][2][128] {maximum, sum} of a tile's rows over 64 keys each
+    static constexpr int Q_AT = RAW_V + RAW;                   // the next segment's queries, f32: 32 columns of all rows, the next 32, ...
+    static constexpr int Q_PART = KP_ROWS * 128;
+    static constexpr int STATS = Q_AT + D / 32 * Q_PART;               // [4][128] {maximum, sum} of a tile's rows
     static constexpr int NOTES = STATS + 4096;
-    static constexpr int BARS = NOTES + KP_NOTES * 128;
+    static constexpr int SCALES = NOTES + KP_NOTES * 128;      // [4][128] powers of two that the queries of a segment were multiplied by (read until its last tile)
+    static constexpr int BARS = SCALES + 4 * KP_ROWS * 4;
     static constexpr int PLAN = BARS + 256;
-    static constexpr int RECORD_ROW = D + 2;
 };
 
 __device__ __forceinline__ void kp_ld16(uint32_t taddr, float (&r)[16]) {
@@ -69,18 +73,19 @@ __device__ __forceinline__ void kp_wait_ld16(float (&r)[16]) {
 }
 
 // Bounded waits without a status word (a role that gives up says so once, at the end): the kernel's loops have to fit the SM's
-// instruction cache together
+// instruction cache together. A probe may sleep for 2 us, or fifteen waiting warps take issue slots from the others.
 __device__ __forceinline__ bool kp_wait(uint32_t bar, uint32_t parity) {
 #pragma unroll 1
-    for (uint32_t i = 0; i < (1u << 22); ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    return false;
-}
-__device__ __forceinline__ bool kp_wait3(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2) {
-#pragma unroll 1
     for (uint32_t i = 0; i < (1u << 22); ++i) {
-        const bool r0 = mbar_try_wait(b0, p0), r1 = mbar_try_wait(b1, p1), r2 = mbar_try_wait(b2, p2);
-        if (r0 & r1 & r2) return true;
+        uint32_t ok;
+        asm volatile(
+            "{\n.reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(2000u)
+            : "memory");
+        if (ok) return true;
     }
     return false;
 }
@@ -209,20 +214,22 @@ struct KpNote {
 static_assert(sizeof(KpNote) == 128, "KP_NOTES of them lie in shared memory");
 
 template <int D>
-__global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvAttention a) {
+__global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ CUtensorMap q_map) {
     using G = KpGeom<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ longlong2 sums[KP_THREADS / 32];
-    __shared__ int run_tiles;
+    __shared__ KpWalk run;                  // the CTA's first tile
+    __shared__ long long run_ends[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int heads[KP_NOTES], begun[KP_NOTES];
+    __shared__ int heads[KP_NOTES], begun[KP_NOTES], segments[KP_NOTES];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = smem_u32(smem), bars = base + G::BARS;
-    // [2] by tile & 1, each used again two tiles later; nfull [KP_NOTES]; from vfull on one phase a tile; from qstaged on one a segment
-    const uint32_t kfull = bars, sfull = bars + 32, pfull = bars + 48, ofull = bars + 64, ofree = bars + 80;
-    const uint32_t nfull = bars + 96, vfull = bars + 160, raw_k = bars + 176, raw_v = bars + 184, raw_k_free = bars + 192;
-    const uint32_t raw_v_free = bars + 200, qstaged = bars + 208, qtaken = bars + 216, qfull = bars + 224, maxima = bars + 232;   // [2] by tile & 1
+    // [2] by tile & 1, each used again two tiles later (pfull: another two for the tile's second 64 keys); nfull [KP_NOTES]; from kfull on one phase a tile; from qstaged on one a segment
+    const uint32_t vfull = bars, sfull = bars + 16, pfull = bars + 32, ofull = bars + 64, ofree = bars + 80;
+    const uint32_t nfull = bars + 96, kfull = bars + 160, raw_k = bars + 176, raw_v = bars + 184, raw_k_free = bars + 192;
+    const uint32_t raw_v_free = bars + 200, qstaged = bars + 216, qtaken = bars + 224, qfull = bars + 232;
     float2 *stats = reinterpret_cast<float2 *>(smem + G::STATS);
+    float *scales = reinterpret_cast<float *>(smem + G::SCALES);
     KpNote *notes = reinterpret_cast<KpNote *>(smem + G::NOTES);
     longlong2 *before = reinterpret_cast<longlong2 *>(smem + G::PLAN);     // [n_seq + 1] places, tiles
     long long *cum = reinterpret_cast<long long *>(before + a.l.n_seq + 1); // [n_seq + 1] places
@@ -230,22 +237,22 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(kfull + i * 8, 4);
+            mbar_init(vfull + i * 8, 4);
             mbar_init(sfull + i * 8, 1);
-            mbar_init(pfull + i * 8, 8);
-            mbar_init(maxima + i * 8, 8);
+            mbar_init(pfull + i * 8, 4);
+            mbar_init(pfull + 16 + i * 8, 4);
             mbar_init(ofull + i * 8, 1);
             mbar_init(ofree + i * 8, 4);
         }
         for (int i = 0; i < KP_NOTES; ++i) mbar_init(nfull + i * 8, 1);
-        mbar_init(vfull, 4);
+        mbar_init(kfull, 4);
         mbar_init(raw_k, 1);
         mbar_init(raw_v, 1);
         mbar_init(raw_k_free, 4);
         mbar_init(raw_v_free, 4);
         mbar_init(qstaged, 1);
-        mbar_init(qtaken, 8);
-        mbar_init(qfull, 8);
+        mbar_init(qtaken, 4);
+        mbar_init(qfull, 4);
         mbar_fence_init();
     }
     if (warp == 0) {
@@ -290,23 +297,26 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     at_fence_before();
     __syncthreads();
     at_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const long long total = before[a.l.n_seq].x, share = (total + gridDim.x - 1) / gridDim.x;
     if (blockIdx.x == 0) {
         for (int i = tid; i <= a.l.n_seq; i += KP_THREADS) a.plan[2 + i] = cum[i];
         if (tid == 0) { a.plan[0] = total; a.plan[1] = share; }
     }
     const long long u0 = min(total, blockIdx.x * share), u1 = min(total, u0 + share);
-    if (warp == 0 && u0 < u1) {
+    if (warp < 2 && u0 < u1) {              // tiles in front of this run and of the next
         KpWalk w;
         int gap;
-        const long long t0 = w.seek(a, cum, QB, u0, gap) + before[w.seq].y;
-        const long long t1 = u1 < total ? w.seek(a, cum, QB, u1, gap) + before[w.seq].y : before[a.l.n_seq].y;
-        if (lane == 0) run_tiles = (int)(t1 - t0);
+        const long long u = warp == 0 ? u0 : u1;
+        long long t = before[a.l.n_seq].y;
+        if (u < total) t = w.seek(a, cum, QB, u, gap) + before[w.seq].y;
+        if (lane == 0) {
+            run_ends[warp] = t;
+            if (warp == 0) run = w;
+        }
     }
-    if (tid == 0 && u0 >= u1) run_tiles = 0;
     __syncthreads();
-    const int n = run_tiles;
+    const int n = u0 < u1 ? (int)(run_ends[1] - run_ends[0]) : 0;
     // TMEM columns: queries (both terms), scores and then weights [2] x 128, weighted values
     const uint32_t t_q = tmem, t_s = tmem + 128, t_o = tmem + 384;
     auto par = [](int i) { return (uint32_t)(i >> 1) & 1u; };
@@ -315,90 +325,98 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         if (warp == 0) {
-            // ---- products, a thread: what it waits for is asked for at once, since a barrier that is ready takes 100 cycles to say so ----
-            if (lane == 0 && n > 0) {
+            // ---- products: what comes last is waited for last, since a barrier that is ready takes 100 cycles to say so ----
+            if (n > 0) {
                 const uint32_t id_s = (1u << 4) | ((uint32_t)(KP_KEYS >> 3) << 17) | ((uint32_t)(KP_ROWS >> 4) << 24);
                 const uint32_t id_o = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(KP_ROWS >> 4) << 24);
                 const uint32_t at = (base >> 4) | 1u << 16;
                 uint32_t segments = 0;
                 auto scores = [&](int i, bool begins) {
                     const int st = i & 1;
-                    if (begins && !kp_wait(qfull, segments++ & 1u)) return false;
-                    // the weights of tile i - 2, which lie where these scores go, have been multiplied
-                    if (i > 1 && !kp_wait(ofull + st * 8, par(i - 2))) return false;
+                    if (begins && !__all_sync(0xffffffffu, kp_wait(qfull, segments++ & 1u))) return false;
                     at_fence_after();
-                    const uint32_t k_at = at + (uint32_t)((G::K_AT + st * G::OPERAND) >> 4);
-#pragma unroll 4
-                    for (int e = 0; e < D / 8; ++e) {           // remainders first
-                        const int kk = e & (D / 16 - 1), term = e < D / 16;
-                        at_mma_ts(t_s + st * 128, t_q + (kk >> 1) * 32 + term * 16 + (kk & 1) * 8, kp_desc(k_at, (kk >> 2) * (KP_KEYS * 128) + (kk & 3) * 32),
-                                  id_s, e > 0);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int e = 0; e < D / 8; ++e) {           // remainders first
+                            const int kk = e & (D / 16 - 1), term = e < D / 16;
+                            at_mma_ts(t_s + st * 128, t_q + (kk >> 1) * 32 + term * 16 + (kk & 1) * 8,
+                                      kp_desc(at, G::K_AT + (kk >> 2) * (KP_KEYS * 128) + (kk & 3) * 32), id_s, e > 0);
+                        }
+                        at_commit(sfull + st * 8);
                     }
-                    at_commit(sfull + st * 8);
+                    __syncwarp();
                     return true;
                 };
                 auto values = [&](int i) {
                     const int st = i & 1;
-                    if (!kp_wait3(vfull, (uint32_t)i & 1u, pfull + st * 8, par(i), i > 0 ? ofree + (st ^ 1) * 8 : vfull,
-                                  i > 0 ? par(i - 1) : (uint32_t)i & 1u)) return false;
-                    at_fence_after();
-#pragma unroll 4
-                    for (int e = 0; e < KP_KEYS / 8; ++e) {
-                        const int kk = e & (KP_KEYS / 16 - 1), term = e < KP_KEYS / 16;
-                        at_mma_ts(t_o, t_s + st * 128 + kk * 16 + term * 8, kp_desc(at, G::V_AT + (kk >> 2) * (D * 128) + (kk & 3) * 32), id_o, e > 0);
+                    if (!__all_sync(0xffffffffu, (i == 0 || kp_wait(ofree + (st ^ 1) * 8, par(i - 1))) && kp_wait(vfull + st * 8, par(i)))) return false;
+                    // as soon as the weights of 64 keys are there: theirs, under the exponentials of the others
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        if (!__all_sync(0xffffffffu, kp_wait(pfull + h * 16 + st * 8, par(i)))) return false;
+                        at_fence_after();
+                        if (elect_one()) {
+                            const uint32_t v_at = at + (uint32_t)((G::V_AT + st * G::OPERAND + h * (D * 128)) >> 4), p_at = t_s + st * 128 + h * 64;
+#pragma unroll
+                            for (int e = 0; e < KP_KEYS / 16; ++e) {
+                                const int kk = e & 3, term = e < 4;
+                                at_mma_ts(t_o, p_at + kk * 16 + term * 8, kp_desc(v_at, kk * 32), id_o, e + h > 0);
+                            }
+                            if (h) at_commit(ofull + st * 8);
+                        }
+                        __syncwarp();
                     }
-                    at_commit(ofull + st * 8);
                     return true;
                 };
-                alive = kp_wait(kfull, 0u) && scores(0, true);
+                alive = __all_sync(0xffffffffu, kp_wait(kfull, 0u)) && scores(0, true);
 #pragma unroll 1
                 for (int i = 0; i < n && alive; ++i) {
-                    // the next tile's scores first, unless its queries still have to take the place of this segment's
-                    bool later = false;
+                    // the next tile's scores first. The weights of tile i - 1, which lie where these scores go, have been multiplied by then
                     if (i + 1 < n) {
-                        alive = kp_wait(kfull + ((i + 1) & 1) * 8, par(i + 1));
+                        const int st = (i + 1) & 1;
+                        alive = __all_sync(0xffffffffu, kp_wait(kfull, (uint32_t)(i + 1) & 1u) && (i == 0 || kp_wait(ofull + st * 8, par(i - 1))));
                         if (!alive) break;
-                        later = begun[(i + 1) % KP_NOTES] != 0;
-                        if (!later) alive = scores(i + 1, false);
+                        alive = scores(i + 1, begun[(i + 1) % KP_NOTES] != 0);
                     }
                     alive = alive && values(i);
-                    if (later) alive = alive && scores(i + 1, true);
                 }
             }
-            __syncwarp();
         } else if (warp == 1 && n > 0) {
-            // ---- queries of the next segment, as they are: a copy a row, 16 bytes apart so that threads can read a row each ----
-            KpWalk w;
-            int gap;
-            w.seek(a, cum, QB, u0, gap);
-            int i = 0, loaded = 1;
+            // ---- queries of the next segment, as they are: one tensor copy per 32 columns of its positions and heads, with the 128-byte
+            // swizzle, so that threads can read a row each (a copy a row took 11,000 cycles, stores of this warp more). Rows behind the
+            // sequence come along and are not looked at ----
+            KpWalk w = run;
+            int i = 0, loaded = 0;
             for (int segment = 0;; ++segment) {
                 if (segment > 0) alive = __all_sync(0xffffffffu, kp_wait(qtaken, (uint32_t)(segment - 1) & 1u));
                 if (!alive) break;
-                const int s0 = w.q * QB, live = min(QB, w.rows - s0) * group;
-                const float *src = a.q + (size_t)(w.row0 + s0) * a.q_stride + (size_t)w.head * group * D;
+                const int s0 = w.q * QB;
                 if (a.wide) {
-                    if (lane == 0) mbar_expect_tx(qstaged, live * D * 4);
+                    if (lane == 0) mbar_expect_tx(qstaged, QB * group * D * 4);
                     __syncwarp();
-                    for (int r = lane; r < live; r += 32)
-                        bulk_load(base + G::Q_AT + r * G::Q_PITCH, src + (size_t)(r / group) * a.q_stride + (size_t)(r % group) * D, D * 4, qstaged);
+                    if (lane < D / 32)
+                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+                                         base + G::Q_AT + lane * G::Q_PART),
+                                     "l"(&q_map), "r"(32 * lane), "r"(w.head * group), "r"(w.row0 + s0), "r"(qstaged)
+                                     : "memory");
                 } else {
+                    const int live = min(QB, w.rows - s0) * group;
                     for (int r = 0; r < live; ++r) {
-                        const float *from = src + (size_t)(r / group) * a.q_stride + (size_t)(r % group) * D;
-                        float *to = reinterpret_cast<float *>(smem + G::Q_AT + r * G::Q_PITCH);
+                        const float *from = a.q + (size_t)(w.row0 + s0 + r / group) * a.q_stride + (size_t)(w.head * group + r % group) * D;
+                        unsigned char *to = smem + G::Q_AT + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
 #pragma unroll
-                        for (int c = 0; c < D; c += 32) to[c + lane] = __ldg(from + c + lane);
+                        for (int c = 0; c < D / 32; ++c) *reinterpret_cast<float *>(to + c * G::Q_PART) = __ldg(from + 32 * c + lane);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(qstaged);
                 }
+                loaded = segment + 1;
                 i += w.t.steps - w.step;
                 if (i >= n) break;
                 w.next_segment(a, QB);
-                loaded = segment + 2;
             }
             // no copy may be in flight when the CTA leaves (bounded)
-            if (!alive) kp_wait(qstaged, (uint32_t)(loaded - 1) & 1u);
+            if (!alive && loaded > 0) kp_wait(qstaged, (uint32_t)(loaded - 1) & 1u);
         } else if (warp > 1 && n > 0) {
             // ---- keys (warp 2) and values (warp 3) as they are cached, by bulk copies; what the others have to know about a tile.
             // Lane g < 8 looks after group g: its page, a tile ahead, and its scales ----
@@ -406,9 +424,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             const int8_t *pool = values ? a.l.v : a.l.k;
             const uint32_t full = values ? raw_v : raw_k, free = values ? raw_v_free : raw_k_free;
             const uint32_t to = base + (values ? G::RAW_V : G::RAW_K) + lane * (KV_GROUP * D);
-            KpWalk w;
-            int gap;
-            w.seek(a, cum, QB, u0, gap);
+            KpWalk w = run;
             const int piece = min(a.l.page / KV_GROUP, 8);        // groups that lie together, from a page's border on
             int id = -1;
             auto page = [&]() {
@@ -420,7 +436,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 }
             };
             bool begins = true;
-            int copied = 0;                                       // tiles on their way or there
+            int segment = 0, copied = 0;                                       // tiles on their way or there
             page();
 #pragma unroll 1
             for (int i = 0; i < n; ++i) {
@@ -463,11 +479,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                         o.begins = begins ? 1 + w.step : 0;
                         o.start = w.start; o.rows = w.rows; o.row0 = w.row0; o.first = w.q * QB;
                         heads[i % KP_NOTES] = w.head;
+                        segments[i % KP_NOTES] = segment;
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(nfull + i % KP_NOTES * 8);
                 }
                 begins = w.step + 1 == w.t.steps;
+                segment += begins;
                 if (i + 1 < n) {
                     w.next(a, QB);
                     page();
@@ -482,79 +500,93 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
         constexpr int ITEMS = KP_KEYS * D / 16 / 128, PER = D == 64 ? 2 : 1;
         const int t = tid - 128, in = t % D, g0 = t / D;
         // (no load from memory may be on its way here: the fence in front of the tensor core would wait for it)
-        // keys a tile ahead of the values, whose place is free only when the product in front has read it: K 0, K 1, V 0, K 2, V 1, ...
+        // (values have two places: in one their conversion, which takes as long as a product, would stand between any two of them)
 #pragma unroll 1
-        for (int j = 0; j < 2 * n + 2; ++j) {
+        for (int j = 0; j < 2 * n; ++j) {
             const bool values = j & 1;
-            const int i = (j >> 1) - values, st = i & 1;
-            if (i < 0 || i >= n) continue;
+            const int i = j >> 1, st = i & 1;
             alive = kp_wait(values ? raw_v : raw_k, (uint32_t)i & 1u);
-            // (keys: the scores of tile i - 2 are there; values: the weighted values of tile i - 1)
-            if (i > 1 - values) alive = alive && kp_wait(values ? ofull + (st ^ 1) * 8 : sfull + st * 8, values ? par(i - 1) : par(i - 2));
+            // (keys: the scores of tile i - 1 are there; values: the weighted values of tile i - 2)
+            if (i > values) alive = alive && kp_wait(values ? ofull + st * 8 : sfull + (st ^ 1) * 8, values ? par(i - 2) : par(i - 1));
             alive = __all_sync(0xffffffffu, alive);
             if (!alive) break;
-            // keys: 16 d of a token are pieces 2 c and 2 c + 1 of its 128-byte row of the 64-d sub-tile. Values: 16 tokens of a row
-            // are pieces 2 (g & 3) and the next of row d of the 64-key half
             const unsigned char *from = smem + (values ? G::RAW_V : G::RAW_K) + t * 16;
-            unsigned char *to = smem + (values ? G::V_AT + in * 128
-                                               : G::K_AT + st * G::OPERAND + (in >> 6) * (KP_KEYS * 128) + (g0 * KV_GROUP + (in & 15)) * 128);
-#pragma unroll 2
-            for (int e = 0; e < ITEMS; ++e) {
-                const int g = e * PER + g0, piece = values ? g & 3 : (in >> 4) & 3;
-                const int at0 = (values ? (g >> 2) * (D * 128) : e * (PER * KV_GROUP * 128)) + (((2 * piece) ^ (in & 7)) << 4);
-                uint4 lo, hi;
-                kp_convert(*reinterpret_cast<const uint4 *>(from + e * 2048), lo, hi);
-                *reinterpret_cast<uint4 *>(to + at0) = lo;
-                *reinterpret_cast<uint4 *>(to + (at0 ^ 16)) = hi;
+            if (values) {   // 16 tokens of a row are pieces 2 (g & 3) and the next of row d of the 64-key half
+                unsigned char *to = smem + G::V_AT + st * G::OPERAND + in * 128;
+                const int swizzle = ((2 * g0) ^ (in & 7)) << 4;
+#pragma unroll
+                for (int e = 0; e < ITEMS; ++e) {
+                    uint4 lo, hi;
+                    kp_convert(*reinterpret_cast<const uint4 *>(from + e * 2048), lo, hi);
+                    const int at0 = (e * PER >> 2) * (D * 128) + (swizzle ^ ((e * PER & 3) << 5));
+                    *reinterpret_cast<uint4 *>(to + at0) = lo;
+                    *reinterpret_cast<uint4 *>(to + (at0 ^ 16)) = hi;
+                }
+            } else {        // 16 d of a token are pieces 2 c and 2 c + 1 of its 128-byte row of the 64-d sub-tile
+                unsigned char *to = smem + G::K_AT + (in >> 6) * (KP_KEYS * 128) + (g0 * KV_GROUP + (in & 15)) * 128;
+                const int at0 = ((2 * ((in >> 4) & 3)) ^ (in & 7)) << 4;
+                unsigned char *to0 = to + at0, *to1 = to + (at0 ^ 16);
+#pragma unroll
+                for (int e = 0; e < ITEMS; ++e) {
+                    uint4 lo, hi;
+                    kp_convert(*reinterpret_cast<const uint4 *>(from + e * 2048), lo, hi);
+                    *reinterpret_cast<uint4 *>(to0 + e * (PER * KV_GROUP * 128)) = lo;
+                    *reinterpret_cast<uint4 *>(to1 + e * (PER * KV_GROUP * 128)) = hi;
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(values ? vfull : kfull + st * 8);
+                mbar_arrive(values ? vfull + st * 8 : kfull);
                 mbar_arrive(values ? raw_v_free : raw_k_free);
             }
         }
     } else if (warp < 16) {
-        // ---- softmax: a thread has 64 keys of a row, warps 8-11 the first of the tile, warps 12-15 the others ----
-        const int half = warp >= 12, row = (warp & 3) * 32 + lane, in_tile = row / group;
+        // ---- softmax, a thread a row: warps 8-11 the even tiles, warps 12-15 the odd ones, so that one tile's exponentials run while
+        // the other's products are waited for ----
+        const int row = (warp & 3) * 32 + lane, in_tile = row / group;
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-        uint32_t segment = 0;
-        float to_log2 = 0.0f;
-        int lim = 0, low = 0;
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
+        for (int i = warp >= 12; i < n; i += 2) {
             const int st = i & 1;
-            const uint32_t s_at = t_s + st * 128 + half * 64 + lane_off;
+            const uint32_t s_at = t_s + st * 128 + lane_off;
             alive = __all_sync(0xffffffffu, kp_wait(nfull + i % KP_NOTES * 8, (uint32_t)(i / KP_NOTES) & 1u));
             if (!alive) break;
             const KpNote &note = notes[i % KP_NOTES];
+            const int segment = segments[i % KP_NOTES], s_pos = note.first + in_tile;
+            const bool there = row < QB * group && s_pos < note.rows;
+            volatile float *scale_at = scales + (segment & 3) * KP_ROWS + row;
             if (note.begins) {
-                // the staged queries take the place of the last segment's, whose scores are done: half the columns each
-                alive = __all_sync(0xffffffffu, kp_wait(qstaged, segment++ & 1u));
+                // its queries take the place of the last segment's, once those scores are done
+                if (i > 0) alive = kp_wait(sfull + (st ^ 1) * 8, par(i - 1));
+                alive = __all_sync(0xffffffffu, alive && kp_wait(qstaged, (uint32_t)segment & 1u));
                 if (!alive) break;
                 at_fence_after();
-                const int s_pos = note.first + in_tile;
-                const bool there = row < QB * group && s_pos < note.rows;
-                const float4 *q = reinterpret_cast<const float4 *>(smem + G::Q_AT + row * G::Q_PITCH);
+                const unsigned char *q = smem + G::Q_AT + row * 128;
+                const int swizzle = (row & 7) << 4;
                 float most = 0.0f;
-#pragma unroll 4
-                for (int j = 0; j < D / 4; ++j) {
-                    const float4 y = q[j];
-                    most = fmaxf(fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 y = *reinterpret_cast<const float4 *>(q + c * G::Q_PART + ((16 * j) ^ swizzle));
+                        most = fmaxf(fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y))), fmaxf(fabsf(y.z), fabsf(y.w)));
+                    }
                 }
                 float up, down;
-                at_scale(there ? most : 0.0f, up, down);
+                at_scale(most, up, down);
+                *scale_at = up;
 #pragma unroll 1
-                for (int j0 = half * (D / 2); j0 < (half + 1) * (D / 2); j0 += 32) {
+                for (int c = 0; c < D / 32; ++c) {
                     uint32_t x[32];               // 16 columns of leading terms, 16 of remainders
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        float4 y = q[j0 / 4 + j];
+                        float4 y = *reinterpret_cast<const float4 *>(q + c * G::Q_PART + ((16 * j) ^ swizzle));
                         if (!there) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         at_split(y.x * up, y.y * up, x[2 * j], x[16 + 2 * j]);
                         at_split(y.z * up, y.w * up, x[2 * j + 1], x[16 + 2 * j + 1]);
                     }
-                    at_st32(t_q + lane_off + j0, x);
+                    at_st32(t_q + lane_off + 32 * c, x);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
                 at_fence_before();
@@ -563,25 +595,28 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                     mbar_arrive(qfull);
                     mbar_arrive(qtaken);
                 }
-                to_log2 = down * a.scale;
-                lim = !there ? 0 : a.causal ? note.start + s_pos + 1 : note.start + note.rows;
-                low = a.window > 0 ? note.start + s_pos + 1 - a.window : 0;
             }
-            const int key0 = note.key0 + half * 64, from = low - key0, to = lim - key0;     // the keys of its 64 that this row sees
-            const float *ks = note.ks + half * 4, *lv = note.lv + half * 4, *iv = note.iv + half * 4;
-            const float4 iv4 = *reinterpret_cast<const float4 *>(iv);
-            const bool edge = __any_sync(0xffffffffu, to < 64 || from > 0 || iv4.x == 0.0f || iv4.y == 0.0f || iv4.z == 0.0f || iv4.w == 0.0f);
+            // the keys of the tile that this row sees (one that is not there sees all, which nobody reads: masks cost time)
+            const int to = !there ? KP_KEYS : (a.causal ? note.start + s_pos + 1 : note.start + note.rows) - note.key0;
+            const int from = a.window > 0 && there ? note.start + s_pos + 1 - a.window - note.key0 : 0;
+            const float *ks = note.ks, *lv = note.lv, *iv = note.iv;
+            // (groups up to the last one that is there, in pairs)
+            const int groups = (32 - __clz(__ballot_sync(0xffffffffu, lane < 8 && iv[lane & 7] != 0.0f)) + 1) & ~1;
+            const bool edge = __any_sync(0xffffffffu, to < KP_KEYS || from > 0 || iv[lane & 7] == 0.0f);
             alive = __all_sync(0xffffffffu, kp_wait(sfull + st * 8, par(i)));
             if (!alive) break;
             at_fence_after();
+            // (the power of two's inverse)
+            const float to_log2 = there ? a.scale * __uint_as_float((254u << 23) - __float_as_uint(*scale_at)) : 0.0f;
             // The loops are kept small: with every role's code laid out flat most of the time went to fetching instructions
             if (edge) {                        // keys that a row does not see
 #pragma unroll 1
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < groups; ++g) {
+                    const bool gone = iv[g] == 0.0f;
+                    if (!__any_sync(0xffffffffu, gone || 16 * g + 16 > to || 16 * g < from)) continue;
                     float v[16];
                     kp_ld16(s_at + 16 * g, v);
                     kp_wait_ld16(v);
-                    const bool gone = iv[g] == 0.0f;
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (gone || 16 * g + e >= to || 16 * g + e < from) v[e] = -INFINITY;
@@ -589,41 +624,38 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             }
-            float mx = -INFINITY;
+            float mx = -INFINITY, v[16], u[16];
+            kp_ld16(s_at, v);
 #pragma unroll 1
-            for (int g = 0; g < 4; g += 2) {
-                float v[16], u[16];
-                kp_ld16(s_at + 16 * g, v);
-                kp_ld16(s_at + 16 * g + 16, u);
-                kp_wait_ld16(v);
-                kp_wait_ld16(u);
-                float x = fmaxf(v[0], v[1]), y = fmaxf(u[0], u[1]);
+            for (int g = 0; g < groups; g += 2) {
+                const float2 k2 = *reinterpret_cast<const float2 *>(ks + g);
+                auto most = [&](const float (&z)[16], float k) {
+                    float x = fmaxf(z[0], z[1]), y = fmaxf(z[2], z[3]);
 #pragma unroll
-                for (int e = 2; e < 16; e += 2) {
-                    x = fmaxf(x, fmaxf(v[e], v[e + 1]));
-                    y = fmaxf(y, fmaxf(u[e], u[e + 1]));
-                }
-                mx = fmaxf(mx, fmaxf(x * (to_log2 * ks[g]), y * (to_log2 * ks[g + 1])));
+                    for (int e = 4; e < 16; e += 4) {
+                        x = fmaxf(x, fmaxf(z[e], z[e + 1]));
+                        y = fmaxf(y, fmaxf(z[e + 2], z[e + 3]));
+                    }
+                    mx = fmaxf(mx, fmaxf(x, y) * (to_log2 * k));
+                };
+                kp_wait_ld16(v);
+                kp_ld16(s_at + 16 * g + 16, u);
+                most(v, k2.x);
+                kp_wait_ld16(u);
+                kp_ld16(s_at + (g + 2 < groups ? 16 * g + 32 : 0), v);     // (at the end the first ones again)
+                most(u, k2.y);
             }
-            // the row's maximum over both halves of the tile; what the output's warps were told last there they have read
-            float2 *mine = stats + (st * 2 + half) * KP_ROWS + row, *other = stats + (st * 2 + (half ^ 1)) * KP_ROWS + row;
-            if (i > 1) alive = __all_sync(0xffffffffu, kp_wait(ofree + st * 8, par(i - 2)));
-            if (!alive) break;
-            mine->x = mx;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(maxima + st * 8);
-            alive = __all_sync(0xffffffffu, kp_wait(maxima + st * 8, par(i)));
-            if (!alive) break;
-            mx = fmaxf(mx, other->x);
             const float off = mx == -INFINITY ? 0.0f : 10.0f - mx;
             float sum = 0.0f;
-#pragma unroll 1
-            for (int g = 0; g < 4; ++g) {
-                float v[16];
-                kp_ld16(s_at + 16 * g, v);
-                const float c = to_log2 * ks[g], og = off + lv[g], inv = iv[g];
+            auto half_done = [&]() {
+                asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+                at_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(pfull + st * 8);
+            };
+            auto weights = [&](int g, const float (&v)[16], float k, float lv, float inv) {
+                const float c = to_log2 * k, og = off + lv;
                 const uint64_t c2 = f2(c, c), og2 = f2(og, og), minus = f2(-1.0f, -1.0f);
-                kp_wait_ld16(v);
                 uint32_t p[16];               // leading terms of 16 weights, remainders
                 uint64_t s2 = 0ull;
 #pragma unroll
@@ -645,30 +677,50 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 float x, y;
                 f2_get(s2, x, y);
                 sum = fmaf(x + y, inv, sum);
+            };
+#pragma unroll 1
+            for (int g = 0; g < groups; g += 2) {
+                if (g == 4) half_done();
+                const float2 k2 = *reinterpret_cast<const float2 *>(ks + g), l2 = *reinterpret_cast<const float2 *>(lv + g), i2 = *reinterpret_cast<const float2 *>(iv + g);
+                kp_wait_ld16(v);
+                kp_ld16(s_at + 16 * g + 16, u);
+                weights(g, v, k2.x, l2.x, i2.x);
+                kp_wait_ld16(u);
+                if (g + 2 < groups) kp_ld16(s_at + 16 * g + 32, v);
+                weights(g + 1, u, k2.y, l2.y, i2.y);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-            mine->y = sum;
+            if (groups == 0) kp_wait_ld16(v);
+#pragma unroll 1
+            for (int g = groups; g < 8; g += 2) {
+                if (g == 4) half_done();
+                const uint32_t none[16] = {};
+                kp_st16(s_at + 16 * g, none);
+                kp_st16(s_at + 16 * g + 16, none);
+            }
+            stats[(i & 3) * KP_ROWS + row] = make_float2(mx, sum);
             at_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(pfull + st * 8);
+            if (lane == 0) mbar_arrive(pfull + 16 + st * 8);
         }
     } else {
         // ---- output ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;\n");
         const int row = (warp & 3) * 32 + lane;
         const uint32_t o_at = t_o + ((uint32_t)((warp & 3) * 32) << 16);
-        unsigned char *stage = smem + G::OUT_AT + (warp & 3) * 4096;
         uint64_t o[D / 2];
         float m = -INFINITY, l = 0.0f;
         bool here = false;                             // here: the segment began in this run
         for (int i = 0; i < n; ++i) {
             const int st = i & 1;
-            alive = __all_sync(0xffffffffu, kp_wait(nfull + i % KP_NOTES * 8, (uint32_t)(i / KP_NOTES) & 1u) &&
-                                                kp_wait(pfull + st * 8, par(i)));
+            // (the note and the rows' statistics were there before. Weights may be a tile ahead by now, so theirs is no barrier to wait on)
+            alive = __all_sync(0xffffffffu, kp_wait(ofull + st * 8, par(i)));
             if (!alive) break;
+            at_fence_after();
+            float t0[16], t1[16];
+            kp_ld16(o_at, t0);
             const KpNote &note = notes[i % KP_NOTES];
-            const float2 ms0 = stats[st * 2 * KP_ROWS + row], ms1 = stats[(st * 2 + 1) * KP_ROWS + row];
-            const float2 ms = make_float2(fmaxf(ms0.x, ms1.x), ms0.y + ms1.y);
+            const float2 ms = stats[(i & 3) * KP_ROWS + row];
             if (note.begins) {
                 here = note.begins == 1;
                 m = -INFINITY;
@@ -682,12 +734,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             m = m_new;
             const float b = beta * fmaxf(note.vmost, 0.0f);
             const uint64_t al2 = f2(alpha, alpha), b2 = f2(b, b);
-            alive = __all_sync(0xffffffffu, kp_wait(ofull + st * 8, par(i)));
-            if (!alive) break;
-            at_fence_after();
             // (read as fast as it goes: the next product with weights waits for it)
-            float t0[16], t1[16];
-            kp_ld16(o_at, t0);
 #pragma unroll
             for (int j0 = 0; j0 < D; j0 += 32) {
                 kp_wait_ld16(t0);
@@ -703,42 +750,31 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             __syncwarp();
             if (lane == 0) mbar_arrive(ofree + st * 8);
             if (note.last) {
-                // ---- the end of a segment, or of this run's part of it, 32 columns at a time through shared memory, so that it
-                // leaves in whole lines ----
+                // ---- the end of a segment, or of this run's part of it: each thread its row, 32 bytes at a time ----
                 const bool whole = here && note.last == 1;
                 const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
                 const uint64_t f_2 = f2(f, f);
-                const int head = heads[i % KP_NOTES];
-                float *rec = a.records + ((size_t)(2 * blockIdx.x + here) * KP_ROWS + (warp & 3) * 32) * G::RECORD_ROW;
-                // (a row of the tile is position rr / group: rr * inverse >> 16, exact for rr below 128)
-                const uint32_t inverse = 65536u / (uint32_t)group + 1u;
-                float *out = a.out + (size_t)(note.row0 + note.first) * a.out_stride + (size_t)head * group * D;
-                const int live = min(QB, note.rows - note.first) * group - (warp & 3) * 32;     // of this warp's rows
+                const int in_tile = row / group;
+                const size_t slot = (size_t)(2 * blockIdx.x + here) * KP_ROWS + row;
+                float *dst = !whole ? a.records + slot * D
+                                    : a.out + (size_t)(note.row0 + note.first + in_tile) * a.out_stride + (size_t)(heads[i % KP_NOTES] * group + row - in_tile * group) * D;
+                if (!whole) reinterpret_cast<float2 *>(a.records + (size_t)2 * gridDim.x * KP_ROWS * D)[slot] = make_float2(m, l);
+                if (row < min(QB, note.rows - note.first) * group) {
 #pragma unroll
-                for (int j0 = 0; j0 < D / 32; ++j0) {
-                    __syncwarp();
+                    for (int j = 0; j < D / 8; ++j) {
+                        float y[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        ulonglong2 y;
-                        y.x = f2_mul(o[16 * j0 + 2 * j], f_2);
-                        y.y = f2_mul(o[16 * j0 + 2 * j + 1], f_2);
-                        *reinterpret_cast<ulonglong2 *>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = y;
-                    }
-                    __syncwarp();
-#pragma unroll 1
-                    for (int r = lane >> 3; r < min(live, 32); r += 4) {
-                        const float4 y = *reinterpret_cast<const float4 *>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-                        const int rr = (warp & 3) * 32 + r, at = (int)((uint32_t)rr * inverse >> 16);
-                        float *p = whole ? out + (size_t)at * a.out_stride + (size_t)(rr - at * group) * D : rec + r * G::RECORD_ROW;
-                        p += 32 * j0 + 4 * (lane & 7);
-                        if (whole && a.wide) {
-                            *reinterpret_cast<float4 *>(p) = y;
+                        for (int e = 0; e < 4; ++e) f2_get(f2_mul(o[4 * j + e], f_2), y[2 * e], y[2 * e + 1]);
+                        if (!whole || a.wide > 1) {
+                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst + 8 * j), "f"(y[0]), "f"(y[1]), "f"(y[2]),
+                                         "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7])
+                                         : "memory");
                         } else {
-                            p[0] = y.x; p[1] = y.y; p[2] = y.z; p[3] = y.w;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) dst[8 * j + e] = y[e];
                         }
                     }
                 }
-                if (!whole) *reinterpret_cast<float2 *>(rec + lane * G::RECORD_ROW + D) = make_float2(m, l);
             }
         }
     }
@@ -757,7 +793,7 @@ template <int D>
 __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_constant__ KvAttention a) {
     pdl_wait();
     pdl_trigger();
-    constexpr int ROW = KpGeom<D>::RECORD_ROW, N = D / 32;
+    constexpr int N = D / 32;
     const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), group = a.group, QB = KP_ROWS / group;
     const long long total = a.plan[0], share = a.plan[1], border = (blockIdx.x + 1) * share;
     if (border >= total) return;
@@ -770,9 +806,10 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
     const int s = w.q * QB + r / group;
     if (r >= QB * group || s >= w.rows) return;
     const int first = blockIdx.x, parts = (int)((to - 1) / share) - first + 1;
-    auto record = [&](int p) { return a.records + ((size_t)(2 * (first + p) + (p == 0)) * KP_ROWS + r) * ROW; };
+    auto slot = [&](int p) { return (size_t)(2 * (first + p) + (p == 0)) * KP_ROWS + r; };
+    const float2 *stats = reinterpret_cast<const float2 *>(a.records + (size_t)2 * (gridDim.x + 1) * KP_ROWS * D);   // (a CTA a border)
     float mx = -INFINITY;
-    for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, record(p)[D]);
+    for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, stats[slot(p)].x);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     const float ref = mx == -INFINITY ? 0.0f : mx;
@@ -780,7 +817,7 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
     for (int p0 = 0; p0 < parts; p0 += 32) {
         float x = 0.0f;
         if (p0 + lane < parts) {
-            const float2 ml = *reinterpret_cast<const float2 *>(record(p0 + lane) + D);
+            const float2 ml = stats[slot(p0 + lane)];
             x = at_exp2(ml.x - ref);
             sum = fmaf(x, ml.y, sum);
         }
@@ -788,7 +825,7 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
 #pragma unroll 8
         for (int p = 0; p < np; ++p) {
             const float y = __shfl_sync(0xffffffffu, x, p);
-            const float *rec = record(p0 + p);
+            const float *rec = a.records + slot(p0 + p) * D;
 #pragma unroll
             for (int e = 0; e < N; ++e) acc[e] = fmaf(y, rec[lane + 32 * e], acc[e]);
         }
@@ -803,19 +840,29 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
 
 // ---- host -----------------------------------------------------------------------------------------
 static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * (sizeof(longlong2) + sizeof(long long)); }
-static size_t kp_plan_bytes(size_t n_seq) { return ((2 + n_seq + 1) * sizeof(long long) + 15) & ~(size_t)15; }
+static size_t kp_plan_bytes(size_t n_seq) { return ((2 + n_seq + 1) * sizeof(long long) + 31) & ~(size_t)31; }
 
 size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head, size_t n_seq) {
-    return kp_plan_bytes(n_seq) + (size_t)2 * ctx->sm_count * KP_ROWS * (d_head + 2) * sizeof(float);
+    return 32 + kp_plan_bytes(n_seq) + (size_t)2 * ctx->sm_count * KP_ROWS * (d_head * sizeof(float) + sizeof(float2));
 }
 bool kv_prompt_takes(size_t d_head, size_t n_seq, size_t group, size_t most_rows) {
     return (d_head == 64 || d_head == 128) && group <= KP_ROWS && most_rows * group > 64 && kp_smem(d_head, n_seq) <= 226 * 1024;
 }
 
-template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a) {
+template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a, size_t rows) {
     auto kern = kv_prompt_kernel<D>;
     if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kern), ctx->device, 226 * 1024)) return rc;
-    YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KP_THREADS), kp_smem(D, a.l.n_seq), ctx->stream, a));
+    CUtensorMap q_map = {};
+    if (a.wide) {
+        const EncodeTiledFn encode = tensor_map_encoder();
+        if (!encode) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "no tensor-map encoder in this driver");
+        const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.n_q, rows}, strides[2] = {(cuuint64_t)D * 4, (cuuint64_t)a.q_stride * 4};
+        const cuuint32_t box[3] = {32, (cuuint32_t)a.group, (cuuint32_t)(KP_ROWS / a.group)}, ones[3] = {1, 1, 1};
+        const CUresult r = encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return fail(YSCV_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
+    }
+    YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KP_THREADS), kp_smem(D, a.l.n_seq), ctx->stream, a, q_map));
     ctx->launches++;
     YSCV_CUDA_TRY(launch_pdl(kv_prompt_merge_kernel<D>, dim3((unsigned)ctx->sm_count - 1, KP_ROWS / 8), dim3(256), 0, ctx->stream, a));
     ctx->launches++;
@@ -824,10 +871,12 @@ template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a) 
     return YSCV_CUDA_OK;
 }
 
-int kv_prompt(yscv_cuda_ctx *ctx, KvAttention a, void *workspace) {
+int kv_prompt(yscv_cuda_ctx *ctx, KvAttention a, void *workspace, size_t rows) {
     a.plan = static_cast<long long *>(workspace);
-    a.records = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kp_plan_bytes(a.l.n_seq));
-    return a.l.d == 64 ? kp_launch<64>(ctx, a) : kp_launch<128>(ctx, a);
+    // (32 bytes at a time: the output's stores)
+    a.records = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + kp_plan_bytes(a.l.n_seq) + 31) & ~(uintptr_t)31);
+    if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 8 == 0) a.wide = 2;
+    return a.l.d == 64 ? kp_launch<64>(ctx, a, rows) : kp_launch<128>(ctx, a, rows);
 }
 
 }  // namespace yscv
