@@ -50,9 +50,10 @@ struct KaSeq {
 __device__ __forceinline__ KaSeq ka_seq(const KvAttention &a, int start, int rows, int R) {
     KaSeq s;
     s.start = start;
-    s.rows = start < 0 ? 0 : max(rows, 0);
+    s.rows = rows;
     s.lo = a.window > 0 ? max(0, start + 1 - a.window) & ~(KA_STEP - 1) : 0;
-    s.steps = s.rows > 0 ? (int)(((long long)start + s.rows - s.lo + KA_STEP - 1) / KA_STEP) : 0;
+    // (positions behind the table's end have no keys; a segment has a step at least)
+    s.steps = s.rows > 0 ? max((min(start, a.room - s.rows) + s.rows - s.lo + KA_STEP - 1) / KA_STEP, 1) : 0;
     s.blocks = (int)(((long long)s.rows * a.group + R - 1) / R);
     return s;
 }
@@ -89,10 +90,10 @@ __device__ __forceinline__ long long ka_plan(const KvAttention &a, int R, long l
     const int per = (n + threads - 1) / threads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
     long long mine = 0;
     for (int i = i0; i < i1; ++i) {
-        const int row0 = a.offsets[i];
-        int2 v = make_int2(a.start[i], a.offsets[i + 1] - row0);
-        const KaSeq s = ka_seq(a, v.x, v.y, R);
-        info[i] = v;
+        const KvSeqRows v = kv_rows(a, i);
+        if (blockIdx.x == 0) kv_rows_status(a, v);
+        const KaSeq s = ka_seq(a, v.start, v.rows, R);
+        info[i] = make_int2(v.start, v.rows);
         cum[i] = mine;
         mine += (long long)s.steps * s.blocks * a.l.n_kv;
     }
@@ -174,8 +175,9 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
     const long long w = (long long)warp * gridDim.x + blockIdx.x, warps = (long long)gridDim.x * G::WARPS;
     const long long share = (total + warps - 1) / warps;
     if (blockIdx.x == 0) {
-        for (int i = tid; i <= a.l.n_seq; i += THREADS) a.plan[2 + i] = cum[i];
-        if (tid == 0) { a.plan[0] = total; a.plan[1] = share; }
+        long long *plan = static_cast<long long *>(a.plan);      // [0] steps, [1] steps of a warp, [2 ..] steps in front of a sequence
+        for (int i = tid; i <= a.l.n_seq; i += THREADS) plan[2 + i] = cum[i];
+        if (tid == 0) { plan[0] = total; plan[1] = share; }
     }
     const long long u0 = w * share, u1 = min(total, u0 + share);
     if (u0 >= u1) return;
@@ -496,9 +498,10 @@ __global__ void __launch_bounds__(32 * W) kv_attention_merge_kernel(const __grid
     __shared__ __align__(8) float part[W][D];
     __shared__ float red[W][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seq = blockIdx.x, head = blockIdx.y;
-    const long long share = a.plan[1], base = a.plan[2 + seq];
-    const int row0 = a.offsets[seq];
-    const KaSeq s = ka_seq(a, a.start[seq], a.offsets[seq + 1] - row0, R);
+    const long long share = static_cast<const long long *>(a.plan)[1], base = static_cast<const long long *>(a.plan)[2 + seq];
+    const KvSeqRows v = kv_rows(a, seq);
+    const int row0 = v.row0;
+    const KaSeq s = ka_seq(a, v.start, v.rows, R);
     if (s.steps == 0) return;
     for (int pair = blockIdx.z; pair < s.rows * a.group; pair += gridDim.z) {
         const int block = pair / R, r = pair - block * R;
@@ -598,8 +601,8 @@ template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttenti
     return YSCV_CUDA_OK;
 }
 
-static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t group, size_t most_rows) {
-    return kv_prompt_takes(pool->d_head, pool->n_seq, group, most_rows) ? kv_prompt_bytes(ctx, pool->d_head, pool->n_seq)
+static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows) {
+    return kv_prompt_takes(pool, group, rows, most_rows) ? kv_prompt_bytes(ctx, pool->d_head, pool->n_seq)
                                                                        : ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * group));
 }
 
@@ -626,7 +629,7 @@ int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_k
                                            size_t *bytes) {
     if (const int rc = ka_check(ctx, pool, n_q, rows, most_rows)) return rc;
     if (!bytes) return fail(YSCV_CUDA_ERR_BAD_ARG, "bytes is null");
-    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, most_rows);
+    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, rows, most_rows);
     return YSCV_CUDA_OK;
 }
 
@@ -643,7 +646,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     if (reinterpret_cast<uintptr_t>(d_workspace) & 15) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the workspace must be 16-byte aligned");
     const size_t group = n_q / pool->n_kv, pairs = most_rows * group;
     const int R = ka_rows(pool->d_head, pairs);
-    const size_t need = attention_bytes(ctx, pool, group, most_rows);
+    const size_t need = attention_bytes(ctx, pool, group, rows, most_rows);
     if (workspace_bytes < need) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     if (rows == 0 || most_rows == 0) return YSCV_CUDA_OK;
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
@@ -659,10 +662,12 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     a.window = (int)(window < (1u << 30) ? window : 0);
     a.wide = ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15) == 0 && q_stride % 4 == 0 && out_stride % 4 == 0;
     a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)pool->d_head)) * 1.4426950408889634f;
-    a.plan = static_cast<long long *>(d_workspace);
+    a.rows = (int)rows;
+    a.room = (int)(pool->max_pages * pool->page);
+    a.plan = d_workspace;
     a.records = reinterpret_cast<float *>(static_cast<unsigned char *>(d_workspace) + ka_plan_bytes(pool->n_seq));
     a.status = ctx->d_status;
-    if (kv_prompt_takes(pool->d_head, pool->n_seq, group, most_rows)) return kv_prompt(ctx, a, d_workspace, rows);
+    if (kv_prompt_takes(pool, group, rows, most_rows)) return kv_prompt(ctx, a, d_workspace);
     switch (pool->d_head) {
         case 64: return R == 8 ? ka_launch<64, 8>(ctx, a, pairs) : ka_launch<64, 16>(ctx, a, pairs);
         case 128: return R == 8 ? ka_launch<128, 8>(ctx, a, pairs) : ka_launch<128, 16>(ctx, a, pairs);

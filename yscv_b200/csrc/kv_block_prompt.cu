@@ -115,7 +115,8 @@ __device__ __forceinline__ void kp_convert(const uint4 &w, uint4 &lo, uint4 &hi)
 }
 
 // ---- where a call's tiles are -----------------------------------------------------------------------
-// Pairs tile q of a sequence: positions q * QB .. ; the keys that any of them sees, from a group's border on
+// Pairs tile q of a sequence: positions q * QB .. ; the keys that any of them sees, from a group's border on. (Positions behind the
+// table's end have no keys; a tile of pairs has a tile of keys at least.)
 struct KpTile {
     int lo, hi, steps;
 };
@@ -123,31 +124,30 @@ __device__ __forceinline__ KpTile kp_tile(const KvAttention &a, int start, int r
     const int s0 = q * QB, s1 = min(rows, s0 + QB);
     KpTile t;
     t.lo = a.window > 0 ? max(0, start + s0 + 1 - a.window) & ~(KV_GROUP - 1) : 0;
-    t.hi = a.causal ? start + s1 : start + rows;
-    t.steps = (t.hi - t.lo + KP_KEYS - 1) / KP_KEYS;
+    t.hi = min(a.causal ? start + s1 : start + rows, a.room);
+    t.steps = max((t.hi - t.lo + KP_KEYS - 1) / KP_KEYS, 1);
     return t;
 }
-__device__ __forceinline__ int kp_tiles(int start, int rows, int QB) { return start < 0 || rows <= 0 ? 0 : (rows + QB - 1) / QB; }
+__device__ __forceinline__ int kp_tiles(int rows, int QB) { return (rows + QB - 1) / QB; }
 // Tiles of a sequence for one KV head, a warp together
-__device__ __forceinline__ long long kp_steps(const KvAttention &a, int start, int rows, int QB) {
-    long long n = 0;
-    for (int q = threadIdx.x & 31; q < kp_tiles(start, rows, QB); q += 32) n += kp_tile(a, start, rows, QB, q).steps;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
+__device__ __forceinline__ int kp_steps(const KvAttention &a, int start, int rows, int QB) {
+    int n = 0;
+    for (int q = threadIdx.x & 31; q < kp_tiles(rows, QB); q += 32) n += kp_tile(a, start, rows, QB, q).steps;
+    return __reduce_add_sync(0xffffffffu, n);
 }
 
 struct KpWalk {
     int seq, q, head, step, start, rows, row0;
     KpTile t;
     __device__ void load(const KvAttention &a) {
-        start = a.start[seq];
-        row0 = a.offsets[seq];
-        rows = a.offsets[seq + 1] - row0;
+        const KvSeqRows r = kv_rows(a, seq);
+        start = r.start;
+        rows = r.rows;
+        row0 = r.row0;
     }
     // The first tile at place u or behind it (u below the last place), a warp together. `at` [n_seq]: places in front of a sequence.
     // Returns the tiles of the sequence in front of it; `gap`: places between u and it.
-    __device__ long long seek(const KvAttention &a, const long long *at, int QB, long long u, int &gap) {
+    __device__ int seek(const KvAttention &a, const int *at, int QB, int u, int &gap) {
         int lo = 0, hi = a.l.n_seq;
         while (hi - lo > 1) {
             const int m = (lo + hi) >> 1;
@@ -156,22 +156,22 @@ struct KpWalk {
         }
         seq = lo;
         load(a);
-        long long left = u - at[seq], tiles = 0;
+        int left = u - at[seq], tiles = 0;
         const int lane = threadIdx.x & 31;
         for (int q0 = 0;; q0 += 32) {
-            const int steps = q0 + lane < kp_tiles(start, rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps : 0;
+            const int steps = q0 + lane < kp_tiles(rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps : 0;
             const int n = steps > 0 ? (steps + KP_BEGIN) * a.l.n_kv : 0;
-            long long upto = n, tiles_upto = (long long)steps * a.l.n_kv;
+            int upto = n, tiles_upto = steps * a.l.n_kv;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, upto, o), z = __shfl_up_sync(0xffffffffu, tiles_upto, o);
+                const int y = __shfl_up_sync(0xffffffffu, upto, o), z = __shfl_up_sync(0xffffffffu, tiles_upto, o);
                 if (lane >= o) { upto += y; tiles_upto += z; }
             }
             const unsigned past = __ballot_sync(0xffffffffu, upto > left);
             if (past) {
                 const int f = __ffs(past) - 1;
                 left -= __shfl_sync(0xffffffffu, upto - n, f);
-                tiles += __shfl_sync(0xffffffffu, tiles_upto - (long long)steps * a.l.n_kv, f);
+                tiles += __shfl_sync(0xffffffffu, tiles_upto - steps * a.l.n_kv, f);
                 q = q0 + f;
                 break;
             }
@@ -179,23 +179,23 @@ struct KpWalk {
             tiles += __shfl_sync(0xffffffffu, tiles_upto, 31);
         }
         t = kp_tile(a, start, rows, QB, q);
-        head = (int)(left / (t.steps + KP_BEGIN));
-        const int in = (int)(left - (long long)head * (t.steps + KP_BEGIN));
+        head = left / (t.steps + KP_BEGIN);
+        const int in = left - head * (t.steps + KP_BEGIN);
         gap = max(0, KP_BEGIN - in);
         step = max(0, in - KP_BEGIN);
-        return tiles + (long long)head * t.steps + step;
+        return tiles + head * t.steps + step;
     }
     // the first step of the next segment (there is one)
     __device__ void next_segment(const KvAttention &a, int QB) {
         step = 0;
         if (++head < a.l.n_kv) return;
         head = 0;
-        if (++q >= kp_tiles(start, rows, QB)) {
+        if (++q >= kp_tiles(rows, QB)) {
             q = 0;
             do {
                 ++seq;
                 load(a);
-            } while (kp_tiles(start, rows, QB) == 0);
+            } while (rows == 0);
         }
         t = kp_tile(a, start, rows, QB, q);
     }
@@ -217,9 +217,9 @@ template <int D>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ CUtensorMap q_map) {
     using G = KpGeom<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ longlong2 sums[KP_THREADS / 32];
+    __shared__ int2 sums[KP_THREADS / 32];
     __shared__ KpWalk run;                  // the CTA's first tile
-    __shared__ long long run_ends[2];
+    __shared__ int run_ends[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int heads[KP_NOTES], begun[KP_NOTES], segments[KP_NOTES];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     float2 *stats = reinterpret_cast<float2 *>(smem + G::STATS);
     float *scales = reinterpret_cast<float *>(smem + G::SCALES);
     KpNote *notes = reinterpret_cast<KpNote *>(smem + G::NOTES);
-    longlong2 *before = reinterpret_cast<longlong2 *>(smem + G::PLAN);     // [n_seq + 1] places, tiles
-    long long *cum = reinterpret_cast<long long *>(before + a.l.n_seq + 1); // [n_seq + 1] places
+    int2 *before = reinterpret_cast<int2 *>(smem + G::PLAN);               // [n_seq + 1] places, tiles
+    int *cum = reinterpret_cast<int *>(before + a.l.n_seq + 1);             // [n_seq + 1] places
     const int group = a.group, QB = KP_ROWS / group;
 
     if (tid == 0) {
@@ -263,30 +263,32 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     pdl_trigger();
     // ---- places and tiles in front of every sequence, and which are this CTA's ----
     for (int i = warp; i < a.l.n_seq; i += KP_THREADS / 32) {
-        const int row0 = a.offsets[i], rows = a.offsets[i + 1] - row0, start = a.start[i];
-        const long long n = kp_steps(a, start, rows, QB);
+        const KvSeqRows r = kv_rows(a, i);
+        const int n = kp_steps(a, r.start, r.rows, QB);
         if (lane == 0) {
-            before[i].y = n * a.l.n_kv;
-            before[i].x = (n + (long long)KP_BEGIN * kp_tiles(start, rows, QB)) * a.l.n_kv;
+            before[i] = make_int2((n + KP_BEGIN * kp_tiles(r.rows, QB)) * a.l.n_kv, n * a.l.n_kv);
+            if (blockIdx.x == 0) kv_rows_status(a, r);
         }
     }
     __syncthreads();
     {
         const int n = a.l.n_seq, per = (n + KP_THREADS - 1) / KP_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-        longlong2 mine = make_longlong2(0, 0);
+        int2 mine = make_int2(0, 0);
         for (int i = i0; i < i1; ++i) { mine.x += before[i].x; mine.y += before[i].y; }
-        longlong2 x = mine;
+        int2 x = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
+            const int y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
             if (lane >= o) { x.x += y; x.y += z; }
         }
         if (lane == 31) sums[warp] = x;
         __syncthreads();
-        longlong2 at = make_longlong2(x.x - mine.x, x.y - mine.y);
-        for (int w = 0; w < warp; ++w) { at.x += sums[w].x; at.y += sums[w].y; }
+        int2 at = make_int2(x.x - mine.x, x.y - mine.y);
+        const int2 w = lane < warp ? sums[lane] : make_int2(0, 0);
+        at.x += __reduce_add_sync(0xffffffffu, w.x);
+        at.y += __reduce_add_sync(0xffffffffu, w.y);
         for (int i = i0; i < i1; ++i) {
-            const longlong2 c = before[i];
+            const int2 c = before[i];
             cum[i] = at.x;
             before[i] = at;
             at.x += c.x;
@@ -298,17 +300,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     __syncthreads();
     at_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-    const long long total = before[a.l.n_seq].x, share = (total + gridDim.x - 1) / gridDim.x;
+    const int total = before[a.l.n_seq].x, share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
     if (blockIdx.x == 0) {
-        for (int i = tid; i <= a.l.n_seq; i += KP_THREADS) a.plan[2 + i] = cum[i];
-        if (tid == 0) { a.plan[0] = total; a.plan[1] = share; }
+        int *plan = static_cast<int *>(a.plan);         // [0] places, [1] places of a CTA, [2 ..] places in front of a sequence
+        for (int i = tid; i <= a.l.n_seq; i += KP_THREADS) plan[2 + i] = cum[i];
+        if (tid == 0) { plan[0] = total; plan[1] = share; }
     }
-    const long long u0 = min(total, blockIdx.x * share), u1 = min(total, u0 + share);
+    const int u0 = min((long long)total, (long long)blockIdx.x * share), u1 = min((long long)total, (long long)u0 + share);
     if (warp < 2 && u0 < u1) {              // tiles in front of this run and of the next
         KpWalk w;
         int gap;
-        const long long u = warp == 0 ? u0 : u1;
-        long long t = before[a.l.n_seq].y;
+        const int u = warp == 0 ? u0 : u1;
+        int t = before[a.l.n_seq].y;
         if (u < total) t = w.seek(a, cum, QB, u, gap) + before[w.seq].y;
         if (lane == 0) {
             run_ends[warp] = t;
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
         }
     }
     __syncthreads();
-    const int n = u0 < u1 ? (int)(run_ends[1] - run_ends[0]) : 0;
+    const int n = u0 < u1 ? run_ends[1] - run_ends[0] : 0;
     // TMEM columns: queries (both terms), scores and then weights [2] x 128, weighted values
     const uint32_t t_q = tmem, t_s = tmem + 128, t_o = tmem + 384;
     auto par = [](int i) { return (uint32_t)(i >> 1) & 1u; };
@@ -795,17 +798,18 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
     pdl_trigger();
     constexpr int N = D / 32;
     const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), group = a.group, QB = KP_ROWS / group;
-    const long long total = a.plan[0], share = a.plan[1], border = (blockIdx.x + 1) * share;
-    if (border >= total) return;
+    const int *plan = static_cast<const int *>(a.plan), total = plan[0], share = plan[1];
+    if ((long long)(blockIdx.x + 1) * share >= total) return;
+    const int border = (blockIdx.x + 1) * share;
     KpWalk w;
     int gap;
-    w.seek(a, a.plan + 2, QB, border, gap);
+    w.seek(a, plan + 2, QB, border, gap);
     // places of the segment's first tile and of the end of its last
-    const long long from = border + gap - w.step, to = from + w.t.steps;
+    const int from = border + gap - w.step, to = from + w.t.steps;
     if (w.step == 0 || from < border - share) return;      // no segment is cut here, or it was cut before
     const int s = w.q * QB + r / group;
     if (r >= QB * group || s >= w.rows) return;
-    const int first = blockIdx.x, parts = (int)((to - 1) / share) - first + 1;
+    const int first = blockIdx.x, parts = (to - 1) / share - first + 1;
     auto slot = [&](int p) { return (size_t)(2 * (first + p) + (p == 0)) * KP_ROWS + r; };
     const float2 *stats = reinterpret_cast<const float2 *>(a.records + (size_t)2 * (gridDim.x + 1) * KP_ROWS * D);   // (a CTA a border)
     float mx = -INFINITY;
@@ -839,24 +843,31 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * (sizeof(longlong2) + sizeof(long long)); }
-static size_t kp_plan_bytes(size_t n_seq) { return ((2 + n_seq + 1) * sizeof(long long) + 31) & ~(size_t)31; }
+static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * (sizeof(int2) + sizeof(int)); }
+static size_t kp_plan_bytes(size_t n_seq) { return ((2 + n_seq + 1) * sizeof(int) + 31) & ~(size_t)31; }
 
 size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head, size_t n_seq) {
     return 32 + kp_plan_bytes(n_seq) + (size_t)2 * ctx->sm_count * KP_ROWS * (d_head * sizeof(float) + sizeof(float2));
 }
-bool kv_prompt_takes(size_t d_head, size_t n_seq, size_t group, size_t most_rows) {
-    return (d_head == 64 || d_head == 128) && group <= KP_ROWS && most_rows * group > 64 && kp_smem(d_head, n_seq) <= 226 * 1024;
+// Above 32 pairs where there are many (sequence, KV head)s, above 64 where there are few, whose SMs have little to do: then this
+// kernel's beginning shows. 8 sequences of 4000 keys, 32 / 4 heads of 64, 5 rows (40 pairs): 27.6 us, 29.3 by steps; 4 rows: 31.4, 26.4.
+// 64 of 2000, 32 / 8 heads of 128, 8 rows (32 pairs): 138, 161. One of 8000, 32 / 4 heads of 64, 8 rows (64 pairs): 26.1, 19.1.
+bool kv_prompt_takes(const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows) {
+    if ((pool->d_head != 64 && pool->d_head != 128) || group > KP_ROWS || kp_smem(pool->d_head, pool->n_seq) > 226 * 1024) return false;
+    // (places are counted in 32 bits)
+    const size_t tiles = rows / (KP_ROWS / group) + pool->n_seq, steps = pool->max_pages * pool->page / KP_KEYS + 2 + KP_BEGIN;
+    if (tiles >= (1u << 31) / pool->n_kv / steps) return false;
+    return most_rows * group > (pool->n_seq * pool->n_kv >= 32 ? 32 : 64);
 }
 
-template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a, size_t rows) {
+template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a) {
     auto kern = kv_prompt_kernel<D>;
     if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kern), ctx->device, 226 * 1024)) return rc;
     CUtensorMap q_map = {};
     if (a.wide) {
         const EncodeTiledFn encode = tensor_map_encoder();
         if (!encode) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "no tensor-map encoder in this driver");
-        const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.n_q, rows}, strides[2] = {(cuuint64_t)D * 4, (cuuint64_t)a.q_stride * 4};
+        const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)a.n_q, (cuuint64_t)a.rows}, strides[2] = {(cuuint64_t)D * 4, (cuuint64_t)a.q_stride * 4};
         const cuuint32_t box[3] = {32, (cuuint32_t)a.group, (cuuint32_t)(KP_ROWS / a.group)}, ones[3] = {1, 1, 1};
         const CUresult r = encode(&q_map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -871,12 +882,12 @@ template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a, 
     return YSCV_CUDA_OK;
 }
 
-int kv_prompt(yscv_cuda_ctx *ctx, KvAttention a, void *workspace, size_t rows) {
-    a.plan = static_cast<long long *>(workspace);
+int kv_prompt(yscv_cuda_ctx *ctx, KvAttention a, void *workspace) {
+    a.plan = workspace;
     // (32 bytes at a time: the output's stores)
     a.records = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + kp_plan_bytes(a.l.n_seq) + 31) & ~(uintptr_t)31);
     if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 8 == 0) a.wide = 2;
-    return a.l.d == 64 ? kp_launch<64>(ctx, a, rows) : kp_launch<128>(ctx, a, rows);
+    return a.l.d == 64 ? kp_launch<64>(ctx, a) : kp_launch<128>(ctx, a);
 }
 
 }  // namespace yscv
