@@ -749,11 +749,12 @@ int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
 /* Attention of the new rows over the pages of one layer: row s of sequence i (q_stride floats apart, n_q
  * heads of d_head, n_q a multiple of n_kv) over the keys 0 .. d_start[i] + s, or all up to the sequence's last new
  * row without `causal`; with window > 0 only over keys after its own position minus window. scale 0
- * stands for 1 / sqrt(d_head). out rows are out_stride floats apart; a row that sees no key is 0.
- * Products are exact in integers: queries and softmax weights enter as three 8-bit digits, cached
- * values as they are. `rows` is the room in d_q and d_out, at least d_offsets[n_seq]. Rows with a NaN or an
- * infinity in the query are NaN, and only those. d_head 64, 128 or 256. _workspace says how many
- * bytes of device memory a call needs; calls that may overlap need one each. */
+ * stands for 1 / sqrt(d_head). out rows are out_stride floats apart and may not overlap d_q; a row that sees no
+ * key is 0. Cached numbers enter the products as they are, queries and softmax weights to 22 bits or more: as three
+ * 8-bit digits and integer products for a few rows a sequence, as two fp16 terms for more. `rows` is the room in d_q and
+ * d_out, at least d_offsets[n_seq]: a sequence whose offsets lie outside takes no part, status 4. Keys behind the table's
+ * end are left out, status 3. Rows with a NaN or an infinity in the query are NaN, and only those. d_head 64, 128 or
+ * 256. _workspace says how many bytes of device memory a call needs; calls that may overlap need one each. */
 int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows,
                                            size_t most_rows, size_t *bytes);
 int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_q,

@@ -618,3 +618,285 @@ def test_copy_of_pages():
         b[:, 7], b[:, 0] = b[:, 3].clone(), b[:, 19].clone()
         assert torch.equal(t, b)
     ctx.close()
+
+
+# ---- the calls that go wrong, and the ones that are easily forgotten --------------------------------
+
+@pytest.mark.parametrize("most", [0, 1, 80])
+def test_attention_serves_the_others_where_a_sequence_s_numbers_are_wrong(most):
+    """Offsets outside the call's rows or falling ones, starts behind the table: told, and nothing beside them changes."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=40, n_kv=1, d=64, page=16, n_seq=3, max_pages=12)
+    pool.give([100, 50, 150])
+    q = torch.randn(6, 4, 64, device="cuda", generator=pool.g)
+    want, tol = attention(pool, q, [98, 48, 148], [2, 2, 2])
+    handle = pool.handle()
+    ws = torch.zeros(ctx.kv_block_attention_workspace(handle, 4, 6, most), dtype=torch.uint8, device="cuda")
+
+    def run(off, start):
+        out = torch.full((8, 4, 64), 3.0, device="cuda")
+        off, start = i32(off), i32(start)
+        torch.cuda.synchronize()
+        ctx.kv_block_attention_dev(handle, 0, q.data_ptr(), 256, 4, off.data_ptr(), start.data_ptr(), 6, most, True, 0, 0.0, out.data_ptr(), 256,
+                                   ws.data_ptr(), ws.numel())
+        ctx.synchronize()
+        assert torch.all(out[6:] == 3.0)
+        return out[:6], ctx.device_status()
+
+    whole, status = run([0, 2, 4, 6], [98, 48, 148])
+    assert status == 0 and torch.all((whole.double() - want).abs() <= tol)
+    # rows that belong to a served sequence alone (the fourth case's last sequence has row 1 too)
+    for off, here in [([0, 2, 4, 7], [0, 1, 2, 3]), ([0, 2, 4, 0x7FFFFFFF], [0, 1, 2, 3]), ([-4, 2, 4, 6], [2, 3, 4, 5]), ([0, 2, 1, 6], [0]),
+                      ([0x7FFFFFFF, -(1 << 31), 4, 6], [4, 5])]:
+        got, status = run(off, [98, 48, 148])
+        assert status == 4
+        assert torch.equal(got[here], whole[here])
+    for start in (0x7FFFFFFF, 0x7FFFFFFE, 12 * 16 - 1, 1 << 24):
+        got, status = run([0, 2, 4, 6], [98, start, 148])
+        assert status in (3, 4) and torch.equal(got[:2], whole[:2]) and torch.equal(got[4:], whole[4:])
+    ctx.close()
+
+
+@pytest.mark.parametrize("d,page,counts,start", [
+    (256, 64, [130, 1, 40], [0, 500, 70]),             # heads of 256 have one kernel for all lengths
+    (128, 128, [129, 256, 3], [127, 0, 128]),          # pages of a tile's size, positions around them
+    (64, 128, [400], [40000]),                         # a piece of a prompt over a long cache, one sequence
+])
+def test_attention_of_longer_rows(d, page, counts, start):
+    ctx = _context()
+    total = [s + m for s, m in zip(start, counts)]
+    pool = Pool(ctx, n_pages=sum(-(-t // page) for t in total) + 2, n_kv=2, d=d, page=page, n_seq=len(start), max_pages=-(-max(total) // page) + 3)
+    pool.give(total)
+    q = torch.randn(sum(counts), 8, d, device="cuda", generator=pool.g)
+    for window in (0, 200):
+        got, live = _attend(ctx, pool, q, counts, start, True, window, scale=0.11)
+        _done(ctx)
+        _check(got, live, *attention(pool, q, start, counts, True, window, 0.11))
+    ctx.close()
+
+
+@pytest.mark.parametrize("rows", [31, 32, 33, 64, 65])
+@pytest.mark.parametrize("n_seq", [1, 40])
+def test_attention_on_both_sides_of_the_choice_of_a_kernel(rows, n_seq):
+    ctx = _context()
+    pool = Pool(ctx, n_pages=n_seq * 7, n_kv=1, d=64, page=32, n_seq=n_seq, max_pages=7)
+    counts, start = [rows] + [i % 3 for i in range(1, n_seq)], [100 + 3 * (i % 5) for i in range(n_seq)]
+    pool.give([s + m for s, m in zip(start, counts)])
+    q = torch.randn(sum(counts), 1, 64, device="cuda", generator=pool.g)
+    got, live = _attend(ctx, pool, q, counts, start)
+    _done(ctx)
+    assert ("tcgen05" in ctx.last_kernel()) == (rows > (64 if n_seq == 1 else 32))
+    _check(got, live, *attention(pool, q, start, counts))
+    ctx.close()
+
+
+def test_pages_behind_two_gigabytes_of_a_layer():
+    """32-bit byte offsets end at page 32768 of these, 32-bit signed ones at 16384."""
+    ctx = _context()
+    page, n_kv, d, n = 64, 8, 128, 33000
+    pool = Pool.__new__(Pool)
+    pool.__dict__.update(ctx=ctx, layers=2, n_pages=n, n_kv=n_kv, d=d, page=page, n_seq=2, max_pages=4, dev="cuda")
+    pool.k = torch.empty(2, n, n_kv, page // 16, d // 16, 16, 16, dtype=torch.int8, device="cuda")
+    pool.v = torch.empty(2, n, n_kv, page // 16, d, 16, dtype=torch.int8, device="cuda")
+    pool.ks, pool.vs = (torch.zeros(2, n, n_kv, device="cuda") for _ in range(2))
+    pool.refs, pool.length = torch.zeros(n, dtype=torch.int32, device="cuda"), i32([0, 0])
+    pool.table = torch.tensor([[n - 1, 7, -1, -1], [16384, n - 2, 16383, -1]], dtype=torch.int32, device="cuda")
+    for p in pool.table.flatten().tolist():
+        if p >= 0:
+            pool.refs[p] = 1
+    g = torch.Generator(device="cuda").manual_seed(3)
+    counts, start = [100, 140], [0, 0]
+    kv = torch.randn(240, 2 * n_kv * d, device="cuda", generator=g)
+    handle, off, st = pool.handle(), offsets(counts), i32(start)
+    torch.cuda.synchronize()
+    for layer in (0, 1):
+        ctx.kv_block_append_dev(handle, layer, kv.data_ptr(), kv[:, n_kv * d:].data_ptr(), 2 * n_kv * d, off.data_ptr(), st.data_ptr(), 140)
+    # another page of the last ones, by a copy
+    src, dst = i32([n - 1]), i32([n - 3])
+    torch.cuda.synchronize()
+    ctx.kv_pages_copy_dev(handle, src.data_ptr(), dst.data_ptr(), 1)
+    _done(ctx)
+    pool.table[0, 0] = n - 3
+    x = kv.view(240, 2, n_kv, d).double()
+    row = 0
+    for i, m in enumerate(counts):
+        for got, want in zip(pool.rows(i, m, 1), (x[row:row + m, 0], x[row:row + m, 1])):
+            # half a step of the scale, which is a 127th of the largest value of a page's head: at most 5.5 / 127
+            assert float((got - want).abs().max()) < 0.5 * 5.5 / 127
+        row += m
+    q = torch.randn(240, 2 * n_kv, d, device="cuda", generator=g)
+    got, live = _attend(ctx, pool, q, counts, start, layer=1)
+    _check(got, live, *attention(pool, q, start, counts, layer=1))
+    got, live = _attend(ctx, pool, q[:2], [1, 1], [99, 139], layer=1)
+    _check(got, live, *attention(pool, q[:2], [99, 139], [1, 1], layer=1))
+    _done(ctx)
+    ctx.close()
+
+
+def test_two_contexts_attend_at_once():
+    """Two streams over one pool, a workspace each, prompts and single tokens, again and again."""
+    ctxs = [_context(), _context()]
+    pool = Pool(ctxs[0], n_pages=80, n_kv=4, d=128, page=32, n_seq=2, max_pages=40)
+    start, counts = [[1000, 700], [400, 100]], [[1, 1], [90, 300]]
+    pool.give([1001, 800])
+    qs = [torch.randn(sum(c), 16, 128, device="cuda", generator=pool.g) for c in counts]
+    offs, sts = [offsets(c) for c in counts], [i32(s) for s in start]
+    outs = [[torch.zeros_like(q) for _ in range(20)] for q in qs]
+    handle = pool.handle()
+    need = [ctxs[0].kv_block_attention_workspace(handle, 16, len(q), max(c)) for q, c in zip(qs, counts)]
+    ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in need]
+    torch.cuda.synchronize()
+    for j in range(20):
+        for i, ctx in enumerate(ctxs):
+            ctx.kv_block_attention_dev(handle, 0, qs[i].data_ptr(), 2048, 16, offs[i].data_ptr(), sts[i].data_ptr(), len(qs[i]), max(counts[i]), True, 0,
+                                       0.0, outs[i][j].data_ptr(), 2048, ws[i].data_ptr(), need[i])
+    for i, ctx in enumerate(ctxs):
+        _done(ctx)
+        want, tol = attention(pool, qs[i], start[i], counts[i])
+        assert torch.all((outs[i][0].double() - want).abs() <= tol)
+        for o in outs[i][1:]:
+            assert torch.equal(o, outs[i][0])
+        ctx.close()
+
+
+class Server:
+    """What a server runs for a step of its sequences, in all layers: pages for the new tokens, then for every layer rotary positions,
+    the cache, attention. The next layer's rows are this one's output, so that a wrong layer shows in all behind it."""
+
+    def __init__(self, stream, n_seq, most, layers=3, n_q=8, n_kv=2, d=64, page=16, n_pages=120, max_pages=30):
+        self.ctx = yscv_b200.Context(0, stream=stream.cuda_stream)
+        self.pool = Pool(self.ctx, layers, n_pages, n_kv, d, page, n_seq, max_pages)
+        self.n_q, self.n_kv, self.d, self.most = n_q, n_kv, d, most
+        self.rows = n_seq * most
+        self.width = (n_q + 2 * n_kv) * d
+        self.rope = yscv_b200.Rope(rotary_dim=d)
+        self.handle = self.pool.handle()
+        self.off, self.start, self.pos = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (n_seq + 1, n_seq, self.rows))
+        self.qkv = torch.zeros(layers, self.rows, self.width, device="cuda")
+        self.turned, self.out = torch.zeros_like(self.qkv), torch.zeros(layers, self.rows, n_q * d, device="cuda")
+        self.work = torch.empty(self.ctx.kv_pages_workspace(self.handle), dtype=torch.uint8, device="cuda")
+        self.ws = torch.empty(self.ctx.kv_block_attention_workspace(self.handle, n_q, self.rows, most), dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+
+    def step(self):
+        ctx, pool, d = self.ctx, self.pool, self.d
+        ctx.kv_pages_extend_dev(self.handle, self.off.data_ptr(), self.rows, self.start.data_ptr(), self.pos.data_ptr(), self.work.data_ptr(),
+                                self.work.numel())
+        for layer in range(pool.layers):
+            x, t = self.qkv[layer], self.turned[layer]
+            ctx.rope_dev(x.data_ptr(), self.width, self.rows, self.n_q + self.n_kv, d, self.pos.data_ptr(), self.rope, t.data_ptr(), self.width)
+            ctx.kv_block_append_dev(self.handle, layer, t[:, self.n_q * d:].data_ptr(), x[:, (self.n_q + self.n_kv) * d:].data_ptr(), self.width,
+                                    self.off.data_ptr(), self.start.data_ptr(), self.most)
+            ctx.kv_block_attention_dev(self.handle, layer, t.data_ptr(), self.width, self.n_q, self.off.data_ptr(), self.start.data_ptr(), self.rows,
+                                       self.most, True, 0, 0.0, self.out[layer].data_ptr(), self.n_q * d, self.ws.data_ptr(), self.ws.numel())
+
+    def check(self, counts, start):
+        """This step's results against the definitions: rotary positions from fp64, the cache as it is now."""
+        n_q, n_kv, d, n = self.n_q, self.n_kv, self.d, sum(counts)
+        pos = np.concatenate([np.arange(s, s + m) if s >= 0 else np.full(m, -1) for s, m in zip(start, counts)]).astype(int)
+        assert self.pos[:n].tolist() == pos.tolist() and torch.all(self.pos[n:] == -1) and self.start.tolist() == [s if m else -1 for s, m in zip(start, counts)]
+        angle = torch.tensor(pos, device="cuda").double()[:, None, None] * torch.tensor(_frequencies(d, "none", 1.0)[0], device="cuda")
+        for layer in range(self.pool.layers):
+            x = self.qkv[layer, :n].double().view(n, -1, d)
+            a, b = x[:, :n_q + n_kv, :d // 2], x[:, :n_q + n_kv, d // 2:]
+            turned = torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], -1)
+            got = self.turned[layer, :n].double().view(n, -1, d)[:, :n_q + n_kv]
+            live = torch.tensor(pos >= 0, device="cuda")
+            # two products, a sum and a sine to 2^-22 of values below 6
+            assert float((got - turned)[live].abs().max()) < 12 * 2.0 ** -22
+            row = 0
+            for i, (s, m) in enumerate(zip(start, counts)):
+                if s >= 0 and m:
+                    for c, w in zip(self.pool.rows(i, s + m, layer), (got[row:row + m, n_q:], x[row:row + m, n_q + n_kv:])):
+                        # a page's scale may grow once per later token of the page, half a step each time, of values below 6
+                        assert float((c[s:] - w).abs().max()) < 16 * 0.5 * 6 / 127
+                row += m
+            want, tol = attention(self.pool, self.turned[layer, :n].view(n, -1, d)[:, :n_q], start, counts, layer=layer)
+            out = self.out[layer, :n].view(n, n_q, d).double()
+            assert torch.all(((out - want).abs() <= tol)[live])
+
+
+def _plan(server, counts, g):
+    """Lays out a step's rows; what runs next on another stream waits for it."""
+    server.off.copy_(offsets(counts))
+    server.qkv.copy_(torch.randn(server.qkv.shape, device="cuda", generator=g))
+    torch.cuda.synchronize()
+
+
+def test_a_server_s_steps():
+    """Prompts, single tokens, drafts and their rejection, branches that share pages, an end, compaction, a prompt in the place that is free."""
+    stream = torch.cuda.Stream()
+    s = Server(stream, n_seq=4, most=70)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    length = [0, 0, 0, 0]
+
+    def go(counts):
+        _plan(s, counts, g)
+        s.step()
+        _done(s.ctx)
+        start = [n if m else -1 for n, m in zip(length, counts)]
+        s.check(counts, start)
+        for i, m in enumerate(counts):
+            length[i] += m
+        assert s.pool.length.tolist() == length
+
+    def lists(call, *rows):
+        rows = [i32(r) for r in rows]
+        torch.cuda.synchronize()
+        call(s.handle, *(r.data_ptr() for r in rows), len(rows[0]))
+        _done(s.ctx)
+
+    go([70, 33, 0, 1])
+    for _ in range(3):
+        go([1, 1, 0, 1])
+    go([5, 4, 0, 70])                                  # drafts beside a piece of a prompt
+    lists(s.ctx.kv_pages_trim_dev, [0, 1], [75, 36])   # of which some were wrong
+    length[0], length[1] = 75, 36
+    lists(s.ctx.kv_pages_fork_dev, [0], [2])           # another branch
+    length[2] = 75
+    for _ in range(18):
+        go([1, 0, 1, 1])
+    lists(s.ctx.kv_pages_trim_dev, [0], [0])           # the first one's end
+    length[0] = 0
+    s.ctx.kv_pages_compact_dev(s.handle, s.work.data_ptr(), s.work.numel())
+    _done(s.ctx)
+    used = int((s.pool.refs > 0).sum())
+    assert torch.all(s.pool.refs[:used] > 0) and int(s.pool.table.max()) == used - 1
+    go([64, 1, 1, 1])
+    go([1, 1, 1, 1])
+    s.ctx.close()
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_a_captured_step_serves_sequences_as_they_grow(most):
+    """One graph, replayed with other offsets and rows while an eager server does the same: bit for bit. Two graphs of one context, with
+    the same workspaces, take turns."""
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    eager, captured = (Server(s, n_seq=3, most=most) for s in streams)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=streams[1], capture_error_mode="thread_local"):
+            captured.step()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for t in range(24):
+        counts = [1 + (t * 7 + i * 5) % most if (t + i) % 4 else 0 for i in range(3)]
+        _plan(eager, counts, g)
+        captured.off.copy_(eager.off)
+        captured.qkv.copy_(eager.qkv)
+        torch.cuda.synchronize()
+        eager.step()
+        with torch.cuda.stream(streams[1]):
+            graphs[t % 2].replay()
+        for s in (eager, captured):
+            s.ctx.synchronize()
+        assert eager.ctx.device_status() == captured.ctx.device_status()
+        n = sum(counts)
+        assert torch.equal(eager.start, captured.start) and torch.equal(eager.pos, captured.pos)
+        assert torch.equal(eager.out[:, :n], captured.out[:, :n])
+        for a, b in zip(eager.pool.state()[4:], captured.pool.state()[4:]):
+            assert torch.equal(a, b)
+    del graphs
+    for s in (eager, captured):
+        s.ctx.close()

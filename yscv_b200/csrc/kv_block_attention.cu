@@ -642,13 +642,14 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     if (!d_q || !d_offsets || !d_start || !d_out || !d_workspace) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
     if (q_stride < n_q * pool->d_head || out_stride < n_q * pool->d_head)
         return fail(YSCV_CUDA_ERR_BAD_ARG, "a row stride is shorter than n_q * d_head");
+    if (d_q == d_out) return fail(YSCV_CUDA_ERR_BAD_ARG, "d_out is d_q");
     if (!(scale >= 0.0f && scale <= FLT_MAX)) return fail(YSCV_CUDA_ERR_BAD_ARG, "scale must be 0 (the default) or positive");
     if (reinterpret_cast<uintptr_t>(d_workspace) & 15) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the workspace must be 16-byte aligned");
-    const size_t group = n_q / pool->n_kv, pairs = most_rows * group;
+    const size_t group = n_q / pool->n_kv, pairs = std::max(most_rows, (size_t)1) * group;   // (a guess of none may be wrong)
     const int R = ka_rows(pool->d_head, pairs);
     const size_t need = attention_bytes(ctx, pool, group, rows, most_rows);
     if (workspace_bytes < need) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
-    if (rows == 0 || most_rows == 0) return YSCV_CUDA_OK;
+    if (rows == 0) return YSCV_CUDA_OK;
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     a.q = d_q;
     a.out = d_out;
