@@ -900,3 +900,116 @@ def test_a_captured_step_serves_sequences_as_they_grow(most):
     del graphs
     for s in (eager, captured):
         s.ctx.close()
+
+
+def _refused(call, *codes):
+    with pytest.raises(yscv_b200.YscvCudaError) as e:
+        call()
+    assert e.value.status in (codes or (-1, -3))
+
+
+def refusals(ctx, dev="cuda"):
+    """Every call that has to be refused, and nothing that is not."""
+    pool = Pool(ctx, layers=2, n_pages=8, n_kv=2, d=64, page=16, n_seq=2, max_pages=4, dev=dev)
+    good = pool.handle()
+    f = torch.zeros(4096, device=dev)
+    n = torch.zeros(64, dtype=torch.int32, device=dev)
+    ws = torch.zeros(1 << 24, dtype=torch.uint8, device=dev)
+    p, i, w = f.data_ptr(), n.data_ptr(), ws.data_ptr()
+    big = 1 << 31
+
+    def calls(h, layer=0, stride=512, k=p, v=p, off=i, start=i, most=1, n_q=4, q=p, out=p + 4096, rows=2, scale=0.0, space=w, size=1 << 24, pos=i, src=i,
+              count=2, seqs=i):
+        return dict(
+            append=lambda: ctx.kv_block_append_dev(h, layer, k, v, stride, off, start, most),
+            read=lambda: ctx.kv_block_read_dev(h, layer, off, start, most, k, v, stride),
+            attend=lambda: ctx.kv_block_attention_dev(h, layer, q, stride, n_q, off, start, rows, most, True, 0, scale, out, stride, space, size),
+            room=lambda: ctx.kv_block_attention_workspace(h, n_q, rows, most),
+            work=lambda: ctx.kv_pages_workspace(h),
+            extend=lambda: ctx.kv_pages_extend_dev(h, off, rows, start, pos, space, size),
+            trim=lambda: ctx.kv_pages_trim_dev(h, seqs, None, count),
+            fork=lambda: ctx.kv_pages_fork_dev(h, src, seqs, count),
+            compact=lambda: ctx.kv_pages_compact_dev(h, space, size),
+            copy=lambda: ctx.kv_pages_copy_dev(h, src, seqs, count))
+
+    def refuse(names, *codes, **change):
+        for name in names.split():
+            _refused(calls(good, **change)[name], *codes)
+
+    every = "append read attend room work extend trim fork compact copy"
+    for change in (dict(d_k=None), dict(d_v=None), dict(d_kscale=None), dict(d_vscale=None), dict(d_refs=None), dict(d_table=None), dict(d_length=None),
+                   dict(layers=0), dict(n_pages=0), dict(n_kv=0), dict(d_head=0), dict(n_seq=0), dict(max_pages=0), dict(page=8), dict(page=48), dict(page=256),
+                   dict(d_head=40), dict(d_head=272), dict(n_pages=1 << 30), dict(n_seq=1 << 20), dict(max_pages=1 << 24), dict(n_kv=1 << 16),
+                   dict(d_k=pool.k.data_ptr() + 8), dict(d_v=pool.v.data_ptr() + 1), dict(d_kscale=pool.ks.data_ptr() + 2), dict(d_refs=pool.refs.data_ptr() + 1),
+                   dict(d_table=pool.table.data_ptr() + 3), dict(d_length=pool.length.data_ptr() + 2)):
+        bad = calls(pool.handle(**change))
+        for name in every.split():
+            _refused(bad[name])
+    refuse("append read attend", -1, layer=2)
+    refuse("append read attend", -1, stride=127)
+    refuse("append read", k=None)
+    refuse("append read", v=None)
+    refuse("append read", -3, k=p + 2)
+    refuse("append read", -3, v=p + 1)
+    refuse("append read attend extend", -1, off=None)
+    refuse("append read attend extend", -1, start=None)
+    refuse("append read attend extend", -3, off=i + 2)
+    refuse("append read attend extend", -3, start=i + 1)
+    refuse("append read attend room", most=big)
+    refuse("attend room", -1, n_q=0)
+    refuse("attend room", -1, n_q=3)
+    refuse("attend room", -3, n_q=65536)
+    refuse("attend room", -3, rows=big // 4)
+    refuse("extend", -3, rows=big)
+    refuse("attend", -1, q=None)
+    refuse("attend", -1, out=None)
+    refuse("attend", -1, out=p)
+    refuse("attend", -3, q=p + 1)
+    refuse("attend", -3, out=p + 4098)
+    for scale in (-1.0, math.inf, math.nan):
+        refuse("attend", -1, scale=scale)
+    refuse("attend extend compact", -1, space=None)
+    refuse("attend extend compact", -1, size=8)
+    refuse("attend", -3, space=w + 8)
+    refuse("extend compact", -3, space=w + 2)
+    refuse("extend", -1, pos=None)
+    refuse("extend", -3, pos=i + 1)
+    refuse("trim fork copy", -1, seqs=None)
+    refuse("trim fork copy", -3, seqs=i + 2)
+    refuse("fork copy", -1, src=None)
+    refuse("fork copy", -3, src=i + 2)
+    refuse("trim fork copy", -3, count=1 << 30)
+    for change in (dict(d_head=48), dict(d_head=16), dict(d_head=192)):
+        for name in ("attend", "room"):
+            _refused(calls(pool.handle(**change))[name], -3)
+    _refused(calls(pool.handle(n_seq=100000, max_pages=16), n_q=2)["room"], -3)
+
+    def rope(x=p, stride=512, rows=2, heads=4, d=64, pos=i, out=p, out_stride=512, **fields):
+        r = yscv_b200.Rope(**{"rotary_dim": 64, **fields})
+        return lambda: ctx.rope_dev(x, stride, rows, heads, d, pos, r, out, out_stride)
+
+    for change in (dict(x=None), dict(pos=None), dict(out=None), dict(x=p + 2), dict(pos=i + 1), dict(out=p + 4098), dict(stride=255), dict(out_stride=255),
+                   dict(out_stride=516), dict(rows=big), dict(heads=0), dict(d=0), dict(rotary_dim=0), dict(rotary_dim=63), dict(rotary_dim=66),
+                   dict(heads=1, d=600, stride=600, out_stride=600, rotary_dim=600), dict(theta=1.0), dict(theta=math.nan), dict(theta=math.inf),
+                   dict(scaling="linear", factor=0.5), dict(scaling="linear", factor=math.nan), dict(scaling="banded", factor=8.0, original_positions=0.0),
+                   dict(scaling="banded", factor=8.0, original_positions=64.0, low_band=4.0, high_band=1.0),
+                   dict(scaling="yarn", factor=8.0, original_positions=64.0, beta_fast=1.0, beta_slow=32.0), dict(attention_factor=-1.0),
+                   dict(attention_factor=math.inf)):
+        _refused(rope(**change))
+    return pool, calls, rope
+
+
+def test_refusals():
+    ctx = _context()
+    torch.cuda.synchronize()
+    pool, calls, rope = refusals(ctx)
+    before = pool.state()
+    # nothing to do is no error, whatever else is missing
+    rope(rows=0, x=None, pos=None, out=None)()
+    for name in ("trim", "fork", "copy"):
+        calls(pool.handle(), count=0, seqs=None, src=None)[name]()
+    calls(pool.handle(), rows=0)["attend"]()
+    _done(ctx)
+    for a, b in zip(pool.state(), before):
+        assert torch.equal(a, b)
+    ctx.close()

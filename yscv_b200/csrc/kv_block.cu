@@ -289,6 +289,7 @@ static int check_rows(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t 
     if (const int rc = kv_check_pool(pool)) return rc;
     if (const int rc = kv_layer_of(pool, layer, l)) return rc;
     if (!d_offsets || !d_start) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_offsets, d_start})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (stride < pool->n_kv * pool->d_head) return fail(YSCV_CUDA_ERR_BAD_ARG, "row stride %zu is shorter than n_kv * d_head", stride);
     if (most_rows >= (1u << 31)) return fail(YSCV_CUDA_ERR_BAD_ARG, "most_rows is too large");
     if (pool->n_seq * (size_t)pages_per_seq(*l, most_rows ? most_rows : 1) >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many pages for one call");
@@ -306,6 +307,7 @@ int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
     KvLayer l;
     if (const int rc = check_rows(ctx, pool, layer, d_offsets, d_start, row_stride, most_rows, &l)) return rc;
     if (!d_k || !d_v) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_k, d_v})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const int per = pages_per_seq(l, most_rows);
     const bool wide = ((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) == 0 && row_stride % 4 == 0;
@@ -329,6 +331,7 @@ int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
     KvLayer l;
     if (const int rc = check_rows(ctx, pool, layer, d_offsets, d_start, row_stride, most_rows, &l)) return rc;
     if (!d_k_out || !d_v_out) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_k_out, d_v_out})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const int per = pages_per_seq(l, most_rows);
     const KvRows rows = {d_offsets, d_start, row_stride};

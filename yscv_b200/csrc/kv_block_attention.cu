@@ -640,6 +640,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     KvAttention a = {};
     if (const int rc = kv_layer_of(pool, layer, &a.l)) return rc;
     if (!d_q || !d_offsets || !d_start || !d_out || !d_workspace) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_q, d_offsets, d_start, d_out})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (q_stride < n_q * pool->d_head || out_stride < n_q * pool->d_head)
         return fail(YSCV_CUDA_ERR_BAD_ARG, "a row stride is shorter than n_q * d_head");
     if (d_q == d_out) return fail(YSCV_CUDA_ERR_BAD_ARG, "d_out is d_q");

@@ -24,6 +24,8 @@ int kv_check_pool(const yscv_cuda_kv_pool *p) {
         return fail(YSCV_CUDA_ERR_UNSUPPORTED, "a size of the pool is too large");
     if ((reinterpret_cast<uintptr_t>(p->d_k) | reinterpret_cast<uintptr_t>(p->d_v)) & 15)
         return fail(YSCV_CUDA_ERR_UNSUPPORTED, "d_k and d_v must be 16-byte aligned");
+    if (!kv_aligned({p->d_kscale, p->d_vscale, p->d_refs, p->d_table, p->d_length}))
+        return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the pool's scales and numbers must be 4-byte aligned");
     return YSCV_CUDA_OK;
 }
 
@@ -465,10 +467,9 @@ static int check_work(const yscv_cuda_kv_pool *p, const void *ws, size_t bytes) 
 
 using namespace yscv;
 
-#define KV_PROLOGUE(ctx, pool)                                             \
-    if (!(ctx)) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null");         \
-    if (const int rc_ = kv_check_pool(pool)) return rc_;                   \
-    YSCV_CUDA_TRY(cudaSetDevice((ctx)->device))
+#define KV_PROLOGUE(ctx, pool)                                     \
+    if (!(ctx)) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null"); \
+    if (const int rc_ = kv_check_pool(pool)) return rc_
 
 extern "C" {
 
@@ -483,8 +484,10 @@ int yscv_cuda_kv_pages_extend_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
                                   int32_t *d_start, int32_t *d_pos, void *d_workspace, size_t workspace_bytes) {
     KV_PROLOGUE(ctx, pool);
     if (!d_offsets || !d_start || (rows > 0 && !d_pos)) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_offsets, d_start, d_pos})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (rows >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows");
     if (const int rc = check_work(pool, d_workspace, workspace_bytes)) return rc;
+    YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const KvWork w = kv_work_of(pool, d_workspace);
     YSCV_CUDA_TRY(launch_pdl(kv_extend_kernel, dim3(1), dim3(KVP_THREADS), 0, ctx->stream, pages_of(pool), d_offsets, d_start, w, ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
@@ -506,7 +509,9 @@ int yscv_cuda_kv_pages_trim_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
     KV_PROLOGUE(ctx, pool);
     if (count == 0) return YSCV_CUDA_OK;
     if (!d_seqs) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_seqs, d_keep})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (count >= (1u << 30)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "list too long");
+    YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const unsigned blocks = (unsigned)((count + 7) / 8 < 4096 ? (count + 7) / 8 : 4096);
     YSCV_CUDA_TRY(launch_pdl(kv_trim_kernel, dim3(blocks), dim3(256), 0, ctx->stream, pages_of(pool), d_seqs, d_keep, (int)count, ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
@@ -520,7 +525,9 @@ int yscv_cuda_kv_pages_fork_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
     KV_PROLOGUE(ctx, pool);
     if (count == 0) return YSCV_CUDA_OK;
     if (!d_src || !d_dst) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_src, d_dst})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (count >= (1u << 20)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "list too long");
+    YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const unsigned blocks = (unsigned)((count + 7) / 8 < 4096 ? (count + 7) / 8 : 4096);
     YSCV_CUDA_TRY(launch_pdl(kv_fork_kernel, dim3(blocks), dim3(256), 0, ctx->stream, pages_of(pool), d_src, d_dst, (int)count, ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
@@ -532,6 +539,7 @@ int yscv_cuda_kv_pages_fork_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
 int yscv_cuda_kv_pages_compact_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, void *d_workspace, size_t workspace_bytes) {
     KV_PROLOGUE(ctx, pool);
     if (const int rc = check_work(pool, d_workspace, workspace_bytes)) return rc;
+    YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const KvWork w = kv_work_of(pool, d_workspace);
     YSCV_CUDA_TRY(launch_pdl(kv_compact_kernel, dim3(1), dim3(KVP_THREADS), 0, ctx->stream, pages_of(pool), w));
     YSCV_CUDA_TRY(cudaGetLastError());
@@ -552,7 +560,9 @@ int yscv_cuda_kv_pages_copy_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
     KV_PROLOGUE(ctx, pool);
     if (count == 0) return YSCV_CUDA_OK;
     if (!d_src || !d_dst) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_src, d_dst})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (count >= (1u << 30)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "list too long");
+    YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     KvApply a = apply_of(pool);
     a.src = d_src;
     a.dst = d_dst;

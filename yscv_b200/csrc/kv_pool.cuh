@@ -7,6 +7,8 @@
 // operand by one bulk copy, bytes as they are, without a swizzle, a transposition or a conversion.
 #pragma once
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "kernels.cuh"
 
@@ -22,6 +24,12 @@ struct KvLayer {
     int n_pages, n_kv, d, page, page_shift, n_seq, max_pages;
 };
 
+// Whether f32 or i32 operands lie where they can be read
+inline bool kv_aligned(std::initializer_list<const void *> operands) {
+    for (const void *p : operands)
+        if (reinterpret_cast<uintptr_t>(p) & 3) return false;
+    return true;
+}
 // Everything about a pool that does not depend on the call: sizes, alignment, null pointers
 int kv_check_pool(const yscv_cuda_kv_pool *p);
 // One layer of a checked pool

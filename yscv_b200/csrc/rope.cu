@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "common.cuh"
+#include "kv_pool.cuh"
 
 namespace yscv {
 
@@ -186,6 +187,7 @@ extern "C" int yscv_cuda_rope_dev(yscv_cuda_ctx *ctx, const float *d_x, size_t x
     int rc = rope_frequencies(rope, a);
     if (rc || rows == 0) return rc;
     if (!d_x || !d_pos || !d_out) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
+    if (!kv_aligned({d_x, d_pos, d_out})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     a.x = d_x; a.out = d_out; a.pos = d_pos; a.x_stride = x_stride; a.out_stride = out_stride;
     a.heads = (int)n_heads; a.d = (int)d_head; a.rot = (int)rope->rotary_dim; a.interleaved = rope->interleaved != 0;
