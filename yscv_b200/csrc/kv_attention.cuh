@@ -44,7 +44,7 @@ __device__ __forceinline__ void kv_rows_status(const KvAttention &a, const KvSeq
 
 // kv_block_prompt.cu: heads of 64 or 128, at most 128 query heads per KV head. `takes` says whether it is the kernel for a call.
 bool kv_prompt_takes(const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows);
-size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head, size_t n_seq);
+size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head);
 int kv_prompt(yscv_cuda_ctx *ctx, KvAttention a, void *workspace);
 
 }  // namespace yscv

@@ -602,7 +602,7 @@ template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttenti
 }
 
 static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows) {
-    return kv_prompt_takes(pool, group, rows, most_rows) ? kv_prompt_bytes(ctx, pool->d_head, pool->n_seq)
+    return kv_prompt_takes(pool, group, rows, most_rows) ? kv_prompt_bytes(ctx, pool->d_head)
                                                                        : ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * group));
 }
 

@@ -145,18 +145,18 @@ struct KpWalk {
         rows = r.rows;
         row0 = r.row0;
     }
-    // The first tile at place u or behind it (u below the last place), a warp together. `at` [n_seq]: places in front of a sequence.
+    // The first tile at place u or behind it (u below the last place), a warp together. `at` [n_seq]: places (.x) in front of a sequence.
     // Returns the tiles of the sequence in front of it; `gap`: places between u and it.
-    __device__ int seek(const KvAttention &a, const int *at, int QB, int u, int &gap) {
+    __device__ int seek(const KvAttention &a, const int2 *at, int QB, int u, int &gap) {
         int lo = 0, hi = a.l.n_seq;
         while (hi - lo > 1) {
             const int m = (lo + hi) >> 1;
-            if (at[m] <= u) lo = m;
+            if (at[m].x <= u) lo = m;
             else hi = m;
         }
         seq = lo;
         load(a);
-        int left = u - at[seq], tiles = 0;
+        int left = u - at[seq].x, tiles = 0;
         const int lane = threadIdx.x & 31;
         for (int q0 = 0;; q0 += 32) {
             const int steps = q0 + lane < kp_tiles(rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps : 0;
@@ -204,6 +204,12 @@ struct KpWalk {
     }
 };
 
+// What a CTA writes down for kv_prompt_merge_kernel about the segment that its run begins within
+struct KpCut {
+    int parts;                     // runs that have a part of it, 0: there is none, or an earlier run says so
+    int row, live, head;           // its first row of the output, its pairs, its KV head
+};
+
 // What warp 2 writes down about a tile for the others
 struct KpNote {
     float ks[8], lv[8], iv[8];     // of its groups: keys' scale; values' scale over the largest one of the tile, log2 and inverse
@@ -232,7 +238,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     float *scales = reinterpret_cast<float *>(smem + G::SCALES);
     KpNote *notes = reinterpret_cast<KpNote *>(smem + G::NOTES);
     int2 *before = reinterpret_cast<int2 *>(smem + G::PLAN);               // [n_seq + 1] places, tiles
-    int *cum = reinterpret_cast<int *>(before + a.l.n_seq + 1);             // [n_seq + 1] places
     const int group = a.group, QB = KP_ROWS / group;
 
     if (tid == 0) {
@@ -289,35 +294,36 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
         at.y += __reduce_add_sync(0xffffffffu, w.y);
         for (int i = i0; i < i1; ++i) {
             const int2 c = before[i];
-            cum[i] = at.x;
             before[i] = at;
             at.x += c.x;
             at.y += c.y;
         }
-        if (tid == KP_THREADS - 1) { cum[n] = at.x; before[n] = at; }
+        if (tid == KP_THREADS - 1) before[n] = at;
     }
     at_fence_before();
     __syncthreads();
     at_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const int total = before[a.l.n_seq].x, share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
-    if (blockIdx.x == 0) {
-        int *plan = static_cast<int *>(a.plan);         // [0] places, [1] places of a CTA, [2 ..] places in front of a sequence
-        for (int i = tid; i <= a.l.n_seq; i += KP_THREADS) plan[2 + i] = cum[i];
-        if (tid == 0) { plan[0] = total; plan[1] = share; }
-    }
     const int u0 = min((long long)total, (long long)blockIdx.x * share), u1 = min((long long)total, (long long)u0 + share);
     if (warp < 2 && u0 < u1) {              // tiles in front of this run and of the next
         KpWalk w;
-        int gap;
+        int gap = 0;
         const int u = warp == 0 ? u0 : u1;
         int t = before[a.l.n_seq].y;
-        if (u < total) t = w.seek(a, cum, QB, u, gap) + before[w.seq].y;
+        if (u < total) t = w.seek(a, before, QB, u, gap) + before[w.seq].y;
         if (lane == 0) {
             run_ends[warp] = t;
-            if (warp == 0) run = w;
+            if (warp == 0) {
+                run = w;
+                // places of the segment's first tile and of the end of its last; cut for the first time?
+                const int from = u0 + gap - w.step, to = from + w.t.steps, s0 = w.q * QB;
+                const bool cut = w.step > 0 && from >= u0 - share;
+                static_cast<KpCut *>(a.plan)[blockIdx.x] = {cut ? (to - 1) / share - (int)blockIdx.x + 2 : 0, w.row0 + s0, min(QB, w.rows - s0) * group, w.head};
+            }
         }
     }
+    if (tid == 0 && u0 >= u1) static_cast<KpCut *>(a.plan)[blockIdx.x].parts = 0;
     __syncthreads();
     const int n = u0 < u1 ? run_ends[1] - run_ends[0] : 0;
     // TMEM columns: queries (both terms), scores and then weights [2] x 128, weighted values
@@ -791,25 +797,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
 }
 
 // Adds the records of segments that several SMs shared: CTAs (border between two runs, eight rows), a warp per row. A segment is
-// merged by its first border.
+// merged by its first border, whose run has written down what it is.
 template <int D>
 __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_constant__ KvAttention a) {
     pdl_wait();
     pdl_trigger();
     constexpr int N = D / 32;
-    const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), group = a.group, QB = KP_ROWS / group;
-    const int *plan = static_cast<const int *>(a.plan), total = plan[0], share = plan[1];
-    if ((long long)(blockIdx.x + 1) * share >= total) return;
-    const int border = (blockIdx.x + 1) * share;
-    KpWalk w;
-    int gap;
-    w.seek(a, plan + 2, QB, border, gap);
-    // places of the segment's first tile and of the end of its last
-    const int from = border + gap - w.step, to = from + w.t.steps;
-    if (w.step == 0 || from < border - share) return;      // no segment is cut here, or it was cut before
-    const int s = w.q * QB + r / group;
-    if (r >= QB * group || s >= w.rows) return;
-    const int first = blockIdx.x, parts = (to - 1) / share - first + 1;
+    const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), group = a.group, first = blockIdx.x;
+    const KpCut cut = static_cast<const KpCut *>(a.plan)[first + 1];
+    const int parts = cut.parts;
+    if (parts == 0 || r >= cut.live) return;
     auto slot = [&](int p) { return (size_t)(2 * (first + p) + (p == 0)) * KP_ROWS + r; };
     const float2 *stats = reinterpret_cast<const float2 *>(a.records + (size_t)2 * (gridDim.x + 1) * KP_ROWS * D);   // (a CTA a border)
     float mx = -INFINITY;
@@ -837,17 +834,17 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float *dst = a.out + (size_t)(w.row0 + s) * a.out_stride + (size_t)(w.head * group + r % group) * D;
+    float *dst = a.out + (size_t)(cut.row + r / group) * a.out_stride + (size_t)(cut.head * group + r % group) * D;
 #pragma unroll
     for (int e = 0; e < N; ++e) dst[lane + 32 * e] = acc[e] * inv;
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * (sizeof(int2) + sizeof(int)); }
-static size_t kp_plan_bytes(size_t n_seq) { return ((2 + n_seq + 1) * sizeof(int) + 31) & ~(size_t)31; }
+static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * sizeof(int2); }
+static size_t kp_plan_bytes(const yscv_cuda_ctx *ctx) { return (ctx->sm_count * sizeof(KpCut) + 31) & ~(size_t)31; }
 
-size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head, size_t n_seq) {
-    return 32 + kp_plan_bytes(n_seq) + (size_t)2 * ctx->sm_count * KP_ROWS * (d_head * sizeof(float) + sizeof(float2));
+size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head) {
+    return 32 + kp_plan_bytes(ctx) + (size_t)2 * ctx->sm_count * KP_ROWS * (d_head * sizeof(float) + sizeof(float2));
 }
 // Above 32 pairs where there are many (sequence, KV head)s, above 64 where there are few, whose SMs have little to do: then this
 // kernel's beginning shows. 8 sequences of 4000 keys, 32 / 4 heads of 64, 5 rows (40 pairs): 27.6 us, 29.3 by steps; 4 rows: 31.4, 26.4.
@@ -885,7 +882,7 @@ template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a) 
 int kv_prompt(yscv_cuda_ctx *ctx, KvAttention a, void *workspace) {
     a.plan = workspace;
     // (32 bytes at a time: the output's stores)
-    a.records = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + kp_plan_bytes(a.l.n_seq) + 31) & ~(uintptr_t)31);
+    a.records = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(workspace) + kp_plan_bytes(ctx) + 31) & ~(uintptr_t)31);
     if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 8 == 0) a.wide = 2;
     return a.l.d == 64 ? kp_launch<64>(ctx, a) : kp_launch<128>(ctx, a);
 }
