@@ -12,6 +12,7 @@
 // byte at a time and an index division per access, 18.5 us.
 #include <cfloat>
 
+#include "attention_tc.cuh"
 #include "kv_pool.cuh"
 
 namespace yscv {
@@ -29,7 +30,7 @@ __device__ __forceinline__ float kv_side(float b, float off) {
 __device__ __forceinline__ bool kv_near_border(float v, float r) { return fabsf(fabsf(v - r) - 0.5f) < 1.220703125e-4f; }
 
 // Whole number nearest to x / s. NaN: 0, infinities: +-127.
-__device__ __forceinline__ int kv_quantise(float x, float s, float inv) {
+__device__ __noinline__ int kv_quantise(float x, float s, float inv) {
     const float v = x * inv;
     float r = rintf(v);
     if (kv_near_border(v, r)) {
@@ -39,31 +40,64 @@ __device__ __forceinline__ int kv_quantise(float x, float s, float inv) {
     r = fminf(fmaxf(r, -127.0f), 127.0f);
     return x == x ? (int)r : 0;
 }
-__device__ __forceinline__ float kv_magnitude(float x) {
-    const float a = fabsf(x);
-    return a <= FLT_MAX ? a : 0.0f;
+// Four quotients' whole numbers, where none is near a border or no number: v + 1.5 * 2^23 rounds v to the nearest one and has it in its
+// low bits (10 instructions for two numbers; rounding and converting instructions and a test of each took 40)
+constexpr float KVB_MAGIC = 12582912.0f;
+__device__ __forceinline__ bool kv_round4(uint64_t v01, uint64_t v23, uint32_t &out) {
+    const uint64_t magic = f2(KVB_MAGIC, KVB_MAGIC), back = f2(-KVB_MAGIC, -KVB_MAGIC), minus = f2(-1.0f, -1.0f);
+    const uint64_t t01 = f2_add(v01, magic), t23 = f2_add(v23, magic);
+    float a, b, c, d, t0, t1, t2, t3;
+    f2_get(f2_fma(f2_add(t01, back), minus, v01), a, b);
+    f2_get(f2_fma(f2_add(t23, back), minus, v23), c, d);
+    f2_get(t01, t0, t1);
+    f2_get(t23, t2, t3);
+    out = __byte_perm(__byte_perm(__float_as_uint(t0), __float_as_uint(t1), 0x0040), __byte_perm(__float_as_uint(t2), __float_as_uint(t3), 0x0040), 0x5410);
+    const float sure = 0.5f - 1.220703125e-4f;
+    return fabsf(a) < sure && fabsf(b) < sure && fabsf(c) < sure && fabsf(d) < sure;
+}
+__device__ __forceinline__ uint32_t kv_quantise4(const float4 &x, float s, float inv) {
+    uint32_t out;
+    if (kv_round4(f2_mul(f2(x.x, x.y), f2(inv, inv)), f2_mul(f2(x.z, x.w), f2(inv, inv)), out)) return out;
+    return (uint32_t)(kv_quantise(x.x, s, inv) & 255) | (uint32_t)(kv_quantise(x.y, s, inv) & 255) << 8 | (uint32_t)(kv_quantise(x.z, s, inv) & 255) << 16 |
+           (uint32_t)(kv_quantise(x.w, s, inv) & 255) << 24;
+}
+// the largest magnitude but for infinities (and NaN, which a maximum passes over)
+__device__ __forceinline__ float kv_most(const float4 &x) {
+    const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    if (m <= FLT_MAX) return m;
+    auto finite = [](float y) { return fabsf(y) <= FLT_MAX ? fabsf(y) : 0.0f; };
+    return fmaxf(fmaxf(finite(x.x), finite(x.y)), fmaxf(finite(x.z), finite(x.w)));
 }
 __device__ __forceinline__ float4 kv_load4(const float *p, bool wide) {
     if (wide) return *reinterpret_cast<const float4 *>(p);
     return make_float4(p[0], p[1], p[2], p[3]);
 }
+// Whole number nearest to q s_old / s_new
+__device__ __noinline__ int kv_requantise1(int q, float ratio, float s_old, float s_new) {
+    const float v = (float)q * ratio;
+    float r = rintf(v);
+    if (kv_near_border(v, r)) {
+        // q s_old - b s_new: the product's rounding apart, the difference of what is left is exact so near the border
+        const float b = floorf(v) + 0.5f, p = (float)q * s_old;
+        r = kv_side(b, fmaf(-b, s_new, p) + fmaf((float)q, s_old, -p));
+    }
+    return (int)r;
+}
 // the first `count` of four numbers, the others as they are
 __device__ __forceinline__ uint32_t kv_requantise(uint32_t w, int count, float ratio, float s_old, float s_new) {
-    uint32_t out = w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i >= count) break;
-        const int q = (int)(int8_t)(w >> (8 * i));
-        const float v = (float)q * ratio;
-        float r = rintf(v);
-        if (kv_near_border(v, r)) {
-            // q s_old - b s_new: the product's rounding apart, the difference of what is left is exact so near the border
-            const float b = floorf(v) + 0.5f, p = (float)q * s_old;
-            r = kv_side(b, fmaf(-b, s_new, p) + fmaf((float)q, s_old, -p));
-        }
-        out = (out & ~(255u << (8 * i))) | (uint32_t)((int)r & 255) << (8 * i);
+    if (count <= 0) return w;
+    // 2^23 + q + 128, less that
+    const uint32_t x = w ^ 0x80808080u, top = 0x4B000000u;
+    const uint64_t off = f2(-8388736.0f, -8388736.0f), by = f2(ratio, ratio);
+    auto number = [&](int sel) { return __uint_as_float(__byte_perm(x, top, sel)); };
+    uint32_t out;
+    if (!kv_round4(f2_mul(f2_add(f2(number(0x7440), number(0x7441)), off), by), f2_mul(f2_add(f2(number(0x7442), number(0x7443)), off), by), out)) {
+        out = 0;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) out |= (uint32_t)(kv_requantise1((int)(int8_t)(w >> (8 * i)), ratio, s_old, s_new) & 255) << (8 * i);
     }
-    return out;
+    const uint32_t mask = count >= 4 ? 0xffffffffu : (1u << (8 * count)) - 1u;
+    return (out & mask) | (w & ~mask);
 }
 
 // Pages of the rows of sequence `seq`: the first and how many
@@ -135,10 +169,9 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
 #pragma unroll
         for (int i = 0; i < KVB_KEEP; ++i)
             if (first + step * i < n)
-                m = fmaxf(m, fmaxf(fmaxf(kv_magnitude(x[i].x), kv_magnitude(x[i].y)), fmaxf(kv_magnitude(x[i].z), kv_magnitude(x[i].w))));
+                m = fmaxf(m, kv_most(x[i]));
         for (int t = first + step * KVB_KEEP; t < n; t += step) {
-            const float4 y = kv_load4(row + (size_t)t * rows.stride, wide);
-            m = fmaxf(m, fmaxf(fmaxf(kv_magnitude(y.x), kv_magnitude(y.y)), fmaxf(kv_magnitude(y.z), kv_magnitude(y.w))));
+            m = fmaxf(m, kv_most(kv_load4(row + (size_t)t * rows.stride, wide)));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -170,9 +203,7 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
         }
         if (tid == 0 && (t0 == 0 || grows)) *scale = s;
         auto put = [&](int t, const float4 &y) {
-            *reinterpret_cast<uint32_t *>(stage + t * pitch + 4 * c) =
-                (uint32_t)(kv_quantise(y.x, s, inv) & 255) | (uint32_t)(kv_quantise(y.y, s, inv) & 255) << 8 |
-                (uint32_t)(kv_quantise(y.z, s, inv) & 255) << 16 | (uint32_t)(kv_quantise(y.w, s, inv) & 255) << 24;
+            *reinterpret_cast<uint32_t *>(stage + t * pitch + 4 * c) = kv_quantise4(y, s, inv);
         };
 #pragma unroll
         for (int i = 0; i < KVB_KEEP; ++i)
