@@ -75,25 +75,22 @@ static KvWork kv_work_of(const yscv_cuda_kv_pool *p, void *ws) {
     return w;
 }
 
-// Exclusive prefix sum over the block's threads, and the sum of all
-__device__ __forceinline__ long long block_prefix(long long v, long long *shared, long long &total) {
+// Exclusive prefix sum over the block's threads, and the sum of all (32 bits hold the pages of all tables)
+__device__ __forceinline__ long long block_prefix(long long v, uint32_t *shared, long long &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
+    uint32_t x = (uint32_t)v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();   // (an earlier sum's readers are done)
     if (lane == 31) shared[warp] = x;
     __syncthreads();
-    long long before = 0;
-    total = 0;
-    for (int w = 0; w < KVP_WARPS; ++w) {
-        if (w < warp) before += shared[w];
-        total += shared[w];
-    }
-    return before + x - v;
+    static_assert(KVP_WARPS == 32, "a lane a warp");
+    const uint32_t w = shared[lane];
+    total = __reduce_add_sync(0xffffffffu, w);
+    return (long long)(__reduce_add_sync(0xffffffffu, lane < warp ? w : 0u) + x - (uint32_t)v);
 }
 
 // Which pages are used, a bit each: of the first KVP_SEEN pages in shared memory, of those behind them looked up again
@@ -171,7 +168,7 @@ constexpr int KVP_LISTED = 2048;   // free pages that are given out from shared 
 
 __global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a, const int32_t *__restrict__ offsets, int32_t *__restrict__ start,
                                                                 const KvWork w, int *__restrict__ status) {
-    __shared__ long long sums[KVP_WARPS];
+    __shared__ uint32_t sums[KVP_WARPS];
     __shared__ uint32_t seen[KVP_SEEN / 32];
     __shared__ int listed[KVP_LISTED];
     __shared__ int copies;
@@ -245,7 +242,7 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a,
 
 // ---- compact --------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(KVP_THREADS) kv_compact_kernel(const KvPages a, const KvWork w) {
-    __shared__ long long sums[KVP_WARPS];
+    __shared__ uint32_t sums[KVP_WARPS];
     __shared__ uint32_t seen[KVP_SEEN / 32];
     pdl_wait();
     pdl_trigger();
