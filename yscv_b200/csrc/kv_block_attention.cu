@@ -488,59 +488,82 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
     }
 }
 
-// Adds the records of a segment that several warps shared: a CTA per (sequence, KV head) and pair, a share of the records for each of
-// its W warps: 16 where there are fewer CTAs than four an SM, else 4 (few records each).
-template <int D, int R, int W>
-__global__ void __launch_bounds__(32 * W) kv_attention_merge_kernel(const __grid_constant__ KvAttention a) {
+// Adds the records of a segment that several warps shared: for each (sequence, KV head) W warps a pair, P pairs a CTA. Either one warp a
+// pair, or, where there are fewer (sequence, head, pair)s than four an SM, sixteen, a share of the records each.
+template <int D, int R, int W, int P>
+__global__ void __launch_bounds__(32 * W * P) kv_attention_merge_kernel(const __grid_constant__ KvAttention a) {
+    static_assert(W == 1 || P == 1, "the shares of a pair are added by its whole CTA");
     pdl_wait();
     pdl_trigger();
-    constexpr int ROW = D + 2, C = D / 32;       // columns of a lane, as pairs: 2 lane + 64 e
+    constexpr int ROW = D + 2, C = D / 64, FIRST = 4;   // pairs of columns of a lane: 2 lane + 64 e
     __shared__ __align__(8) float part[W][D];
     __shared__ float red[W][2];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seq = blockIdx.x, head = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = W == 1 ? 0 : tid >> 5, seq = blockIdx.x, head = blockIdx.y;
     const long long share = static_cast<const long long *>(a.plan)[1], base = static_cast<const long long *>(a.plan)[2 + seq];
     const KvSeqRows v = kv_rows(a, seq);
     const int row0 = v.row0;
     const KaSeq s = ka_seq(a, v.start, v.rows, R);
     if (s.steps == 0) return;
-    for (int pair = blockIdx.z; pair < s.rows * a.group; pair += gridDim.z) {
+    for (int pair = blockIdx.z * P + (W == 1 ? tid >> 5 : 0); pair < s.rows * a.group; pair += gridDim.z * P) {
         const int block = pair / R, r = pair - block * R;
         const long long from = base + ((long long)head * s.blocks + block) * s.steps, to = from + s.steps;
         const long long wa = from / share, wb = (to - 1) / share;
         if (wa == wb) continue;                  // one warp had it all and wrote it
         const int parts = (int)(wb - wa) + 1;
         auto record = [&](int p) { return a.records + ((size_t)(2 * (wa + p) + (p == 0)) * R + r) * ROW; };
-        // every warp its records, 32 at a time, by its own maximum
-        float m = -INFINITY, l = 0.0f, acc[C] = {};
+        // every warp its records, 32 at a time, by its own maximum; the first ones are fetched beside their maxima and sums
+        float m = -INFINITY, l = 0.0f;
+        uint64_t acc[C] = {}, x[FIRST][C];
         for (int p0 = warp; p0 < parts; p0 += 32 * W) {
             const int mine = p0 + W * lane, np = min(32, (parts - p0 + W - 1) / W);
             float2 ml = make_float2(-INFINITY, 0.0f);
             if (mine < parts) ml = *reinterpret_cast<const float2 *>(record(mine) + D);
+            auto fetch = [&](int p, uint64_t (&y)[C]) {
+                const float *rec = record(p0 + W * min(p, np - 1)) + 2 * lane;
+#pragma unroll
+                for (int e = 0; e < C; ++e) y[e] = *reinterpret_cast<const uint64_t *>(rec + 64 * e);
+            };
+#pragma unroll
+            for (int p = 0; p < FIRST; ++p) fetch(p, x[p]);
             float mx = ml.x;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float old = ka_exp2(m - ref), w = ka_exp2(ml.x - ref);
+            const float old = ka_exp2(m - ref), w = ka_exp2(ml.x - ref);   // (0 for a lane without a record)
             m = m_new;
             l = fmaf(l, old, w * ml.y);          // (of the lane's records)
 #pragma unroll
-            for (int e = 0; e < C; ++e) acc[e] *= old;
-#pragma unroll 8
-            for (int p = 0; p < np; ++p) {
-                const float y = __shfl_sync(0xffffffffu, w, p);
-                const float *rec = record(p0 + W * p) + 2 * lane;
+            for (int e = 0; e < C; ++e) acc[e] = f2_mul(acc[e], f2(old, old));
+            for (int p = 0; p < np; p += FIRST) {
 #pragma unroll
-                for (int e = 0; e < C / 2; ++e) {
-                    const float2 v = *reinterpret_cast<const float2 *>(rec + 64 * e);
-                    acc[2 * e] = fmaf(y, v.x, acc[2 * e]);
-                    acc[2 * e + 1] = fmaf(y, v.y, acc[2 * e + 1]);
+                for (int q = 0; q < FIRST; ++q) {
+                    const float y = __shfl_sync(0xffffffffu, w, min(p + q, 31));
+                    if (p + q < np)
+#pragma unroll
+                        for (int e = 0; e < C; ++e) acc[e] = f2_fma(f2(y, y), x[q][e], acc[e]);
                 }
+                if (p + FIRST < np)
+#pragma unroll
+                    for (int q = 0; q < FIRST; ++q) fetch(p + FIRST + q, x[q]);
             }
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        const int sq = pair / a.group;
+        float *dst = a.out + (size_t)(row0 + sq) * a.out_stride + (size_t)(head * a.group + pair - sq * a.group) * D;
+        if (W == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int e = 0; e < C / 2; ++e) *reinterpret_cast<float2 *>(&part[warp][2 * lane + 64 * e]) = make_float2(acc[2 * e], acc[2 * e + 1]);
+            for (int e = 0; e < C; ++e) {
+                float2 y;
+                f2_get(f2_mul(acc[e], f2(inv, inv)), y.x, y.y);
+                dst[2 * lane + 64 * e] = y.x;
+                dst[2 * lane + 64 * e + 1] = y.y;
+            }
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < C; ++e) *reinterpret_cast<uint64_t *>(&part[warp][2 * lane + 64 * e]) = acc[e];
         if (lane == 0) { red[warp][0] = m; red[warp][1] = l; }
         __syncthreads();
         float all = red[0][0];
@@ -551,13 +574,11 @@ __global__ void __launch_bounds__(32 * W) kv_attention_merge_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < W; ++i) sum = fmaf(ka_exp2(red[i][0] - ref), red[i][1], sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int sq = pair / a.group;
-        float *dst = a.out + (size_t)(row0 + sq) * a.out_stride + (size_t)(head * a.group + pair - sq * a.group) * D;
         for (int c = tid; c < D; c += 32 * W) {
-            float x = 0.0f;
+            float y = 0.0f;
 #pragma unroll
-            for (int i = 0; i < W; ++i) x = fmaf(ka_exp2(red[i][0] - ref), part[i][c], x);
-            dst[c] = x * inv;
+            for (int i = 0; i < W; ++i) y = fmaf(ka_exp2(red[i][0] - ref), part[i][c], y);
+            dst[c] = y * inv;
         }
         __syncthreads();
     }
@@ -591,10 +612,10 @@ template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttenti
     if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void *>(kern), ctx->device, 226 * 1024)) return rc;
     YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KaGeom<D, R>::WARPS * 32), ka_smem(D, R, a.l.n_seq), ctx->stream, a));
     ctx->launches++;
-    const unsigned z = (unsigned)(pairs < 1024 ? pairs : 1024);
+    const size_t z = pairs < 1024 ? pairs : 1024;
     const bool few = (size_t)a.l.n_seq * a.l.n_kv * z < (size_t)4 * ctx->sm_count;
-    YSCV_CUDA_TRY(launch_pdl(few ? kv_attention_merge_kernel<D, R, 16> : kv_attention_merge_kernel<D, R, 4>,
-                             dim3((unsigned)a.l.n_seq, (unsigned)a.l.n_kv, z), dim3(few ? 512 : 128), 0, ctx->stream, a));
+    YSCV_CUDA_TRY(launch_pdl(few ? kv_attention_merge_kernel<D, R, 16, 1> : kv_attention_merge_kernel<D, R, 1, 8>,
+                             dim3((unsigned)a.l.n_seq, (unsigned)a.l.n_kv, (unsigned)(few ? z : (z + 7) / 8)), dim3(few ? 512 : 256), 0, ctx->stream, a));
     ctx->launches++;
     YSCV_CUDA_TRY(cudaGetLastError());
     ctx->last_kernel = "kv_block_attention(steps,imma)";
