@@ -685,7 +685,7 @@ def test_attention_on_both_sides_of_the_choice_of_a_kernel(rows, n_seq):
     q = torch.randn(sum(counts), 1, 64, device="cuda", generator=pool.g)
     got, live = _attend(ctx, pool, q, counts, start)
     _done(ctx)
-    assert ("tcgen05" in ctx.last_kernel()) == (rows > (64 if n_seq == 1 else 32))
+    assert ("tcgen05" in ctx.last_kernel()) == (rows > 32)
     _check(got, live, *attention(pool, q, start, counts))
     ctx.close()
 

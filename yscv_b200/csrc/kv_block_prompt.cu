@@ -22,7 +22,7 @@
 // Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, with room for KP_BEGIN tiles in front of each
 // segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
 // kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and causal prompts, whose first
-// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 174 us; an earlier form with longer beginnings took
+// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 165 us; an earlier form with longer beginnings took
 // 456 us with tiles alone and 210 with room for two).
 // Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128; what holds a tile for 3600
 // is the chain of its two products and its softmax, with as many tiles on their way as TMEM has room for (two), and the issue slots,
@@ -846,15 +846,19 @@ static size_t kp_plan_bytes(const yscv_cuda_ctx *ctx) { return (ctx->sm_count * 
 size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head) {
     return 32 + kp_plan_bytes(ctx) + (size_t)2 * ctx->sm_count * KP_ROWS * (d_head * sizeof(float) + sizeof(float2));
 }
-// Above 32 pairs where there are many (sequence, KV head)s, above 64 where there are few, whose SMs have little to do: then this
-// kernel's beginning shows. 8 sequences of 4000 keys, 32 / 4 heads of 64, 5 rows (40 pairs): 27.6 us, 29.3 by steps; 4 rows: 31.4, 26.4.
-// 64 of 2000, 32 / 8 heads of 128, 8 rows (32 pairs): 138, 161. One of 8000, 32 / 4 heads of 64, 8 rows (64 pairs): 26.1, 19.1.
+// Above 32 pairs a KV head, which the other kernel takes as two blocks of 16 that read the cache once each (us here, by steps):
+//                                                   heads of 128, group 4                  heads of 64, group 8
+//   pairs                                           16          32          64             32          64
+//   8 sequences of 300 keys, 32 query heads         18.6, 20.8  19.0, 19.8  19.8, 28.3     15.2, 15.8  15.3, 16.5
+//   8 of 4000                                       43.4, 39.4  44.0, 47.1  45.2, 76.7     26.8, 27.8  26.5, 36.1
+//   64 of 2000                                      128, 89     131, 147    136, 265       61, 55      63, 89
+//   one of 8000                                     26.4, 21.6  26.8, 24.2  27.6, 37.7     19.2, 16.4  19.6, 18.4
 bool kv_prompt_takes(const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows) {
     if ((pool->d_head != 64 && pool->d_head != 128) || group > KP_ROWS || kp_smem(pool->d_head, pool->n_seq) > 226 * 1024) return false;
     // (places are counted in 32 bits)
     const size_t tiles = rows / (KP_ROWS / group) + pool->n_seq, steps = pool->max_pages * pool->page / KP_KEYS + 2 + KP_BEGIN;
     if (tiles >= (1u << 31) / pool->n_kv / steps) return false;
-    return most_rows * group > (pool->n_seq * pool->n_kv >= 32 ? 32 : 64);
+    return most_rows * group > 32;
 }
 
 template <int D> static int kp_launch(yscv_cuda_ctx *ctx, const KvAttention &a) {
