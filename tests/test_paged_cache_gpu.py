@@ -675,6 +675,24 @@ def test_attention_of_longer_rows(d, page, counts, start):
     ctx.close()
 
 
+@pytest.mark.parametrize("most", [1, 70])
+def test_attention_of_pages_whose_scales_are_zero(most):
+    """Keys of 0 take part with a score of 0, values of 0 with their weight: beside others, and alone."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=40, n_kv=1, d=64, page=16, n_seq=2, max_pages=20)
+    pool.give([200, 150])
+    pages = pool.table[0].long()
+    pool.vs[:, pages[2:5]] = 0.0
+    pool.ks[:, pages[4:7]] = 0.0
+    pool.vs[:, pool.table[1, :10].long()] = 0.0
+    q = torch.randn(2, 4, 64, device="cuda", generator=pool.g)
+    got, live = _attend(ctx, pool, q, [1, 1], [199, 149], most=most)
+    _done(ctx)
+    _check(got, live, *attention(pool, q, [199, 149], [1, 1]))
+    assert torch.all(got[1] == 0)
+    ctx.close()
+
+
 @pytest.mark.parametrize("rows", [31, 32, 33, 64, 65])
 @pytest.mark.parametrize("n_seq", [1, 40])
 def test_attention_on_both_sides_of_the_choice_of_a_kernel(rows, n_seq):

@@ -477,9 +477,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
 #pragma unroll
                     for (int d = 4; d > 0; d >>= 1) vmost = fmaxf(vmost, __shfl_xor_sync(0xffffffffu, vmost, d));
                     if (lane < 8) {
+                        // (at least 2^-60: a group whose values are 0 counts in the sum all the same)
+                        const float ratio = fmaxf(__fdiv_rn(vs, fmaxf(vmost, 7.5e-37f)), 8.6736174e-19f);
                         o.ks[lane] = ks;
-                        o.lv[lane] = there ? (vs == vmost ? 0.0f : log2f(__fdiv_rn(vs, vmost))) : -INFINITY;
-                        o.iv[lane] = there ? __fdiv_rn(vmost, vs) : 0.0f;
+                        o.lv[lane] = there ? log2f(ratio) : -INFINITY;
+                        o.iv[lane] = there ? __fdiv_rn(1.0f, ratio) : 0.0f;
                     }
                     if (lane == 0) {
                         o.vmost = vmost;
