@@ -145,18 +145,11 @@ struct KpWalk {
         rows = r.rows;
         row0 = r.row0;
     }
-    // The first tile at place u or behind it (u below the last place), a warp together. `at` [n_seq]: places (.x) in front of a sequence.
-    // Returns the tiles of the sequence in front of it; `gap`: places between u and it.
-    __device__ int seek(const KvAttention &a, const int2 *at, int QB, int u, int &gap) {
-        int lo = 0, hi = a.l.n_seq;
-        while (hi - lo > 1) {
-            const int m = (lo + hi) >> 1;
-            if (at[m].x <= u) lo = m;
-            else hi = m;
-        }
-        seq = lo;
+    // The first tile at place `left` of sequence `seq` or behind it (there is one), a warp together. Returns the tiles of the sequence in
+    // front of it; `gap`: places between the two.
+    __device__ int seek(const KvAttention &a, int QB, int left, int &gap) {
         load(a);
-        int left = u - at[seq].x, tiles = 0;
+        int tiles = 0;
         const int lane = threadIdx.x & 31;
         for (int q0 = 0;; q0 += 32) {
             const int steps = q0 + lane < kp_tiles(rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps : 0;
@@ -223,7 +216,6 @@ template <int D>
 __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_constant__ KvAttention a, const __grid_constant__ CUtensorMap q_map) {
     using G = KpGeom<D>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ int2 sums[KP_THREADS / 32];
     __shared__ KpWalk run;                  // the CTA's first tile
     __shared__ int run_ends[2];
     __shared__ uint32_t tmem_slot;
@@ -237,7 +229,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     float2 *stats = reinterpret_cast<float2 *>(smem + G::STATS);
     float *scales = reinterpret_cast<float *>(smem + G::SCALES);
     KpNote *notes = reinterpret_cast<KpNote *>(smem + G::NOTES);
-    int2 *before = reinterpret_cast<int2 *>(smem + G::PLAN);               // [n_seq + 1] places, tiles
+    int2 *counted = reinterpret_cast<int2 *>(smem + G::PLAN);               // [n_seq] places and tiles
     const int group = a.group, QB = KP_ROWS / group;
 
     if (tid == 0) {
@@ -266,66 +258,68 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     }
     pdl_wait();
     pdl_trigger();
-    // ---- places and tiles in front of every sequence, and which are this CTA's ----
+    // ---- places and tiles of every sequence, and which are this CTA's ----
     for (int i = warp; i < a.l.n_seq; i += KP_THREADS / 32) {
         const KvSeqRows r = kv_rows(a, i);
         const int n = kp_steps(a, r.start, r.rows, QB);
         if (lane == 0) {
-            before[i] = make_int2((n + KP_BEGIN * kp_tiles(r.rows, QB)) * a.l.n_kv, n * a.l.n_kv);
+            counted[i] = make_int2((n + KP_BEGIN * kp_tiles(r.rows, QB)) * a.l.n_kv, n * a.l.n_kv);
             if (blockIdx.x == 0) kv_rows_status(a, r);
         }
-    }
-    __syncthreads();
-    {
-        const int n = a.l.n_seq, per = (n + KP_THREADS - 1) / KP_THREADS, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-        int2 mine = make_int2(0, 0);
-        for (int i = i0; i < i1; ++i) { mine.x += before[i].x; mine.y += before[i].y; }
-        int2 x = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
-            if (lane >= o) { x.x += y; x.y += z; }
-        }
-        if (lane == 31) sums[warp] = x;
-        __syncthreads();
-        int2 at = make_int2(x.x - mine.x, x.y - mine.y);
-        const int2 w = lane < warp ? sums[lane] : make_int2(0, 0);
-        at.x += __reduce_add_sync(0xffffffffu, w.x);
-        at.y += __reduce_add_sync(0xffffffffu, w.y);
-        for (int i = i0; i < i1; ++i) {
-            const int2 c = before[i];
-            before[i] = at;
-            at.x += c.x;
-            at.y += c.y;
-        }
-        if (tid == KP_THREADS - 1) before[n] = at;
     }
     at_fence_before();
     __syncthreads();
     at_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-    const int total = before[a.l.n_seq].x, share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
-    const int u0 = min((long long)total, (long long)blockIdx.x * share), u1 = min((long long)total, (long long)u0 + share);
-    if (warp < 2 && u0 < u1) {              // tiles in front of this run and of the next
+    if (warp < 2) {                         // where this run begins, and where the next does
+        const int n_seq = a.l.n_seq;
+        auto counts = [&](int i0) { return i0 + lane < n_seq ? counted[i0 + lane] : make_int2(0, 0); };
+        int total = 0, t = 0;               // places of the call; tiles in front of place u
+        for (int i0 = 0; i0 < n_seq; i0 += 32) {
+            const int2 c = counts(i0);
+            total += __reduce_add_sync(0xffffffffu, c.x);
+            t += __reduce_add_sync(0xffffffffu, c.y);
+        }
+        const int share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x), u0 = (int)min((long long)total, (long long)blockIdx.x * share);
+        const int u = warp == 0 ? u0 : (int)min((long long)total, (long long)u0 + share);
         KpWalk w;
         int gap = 0;
-        const int u = warp == 0 ? u0 : u1;
-        int t = before[a.l.n_seq].y;
-        if (u < total) t = w.seek(a, before, QB, u, gap) + before[w.seq].y;
+        if (u < total) {
+            int i0 = 0, front = 0;
+            t = 0;
+            int2 c = counts(0);
+            for (int x; (x = __reduce_add_sync(0xffffffffu, c.x)) <= u - front; c = counts(i0 += 32)) {
+                front += x;
+                t += __reduce_add_sync(0xffffffffu, c.y);
+            }
+            int2 x = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
+                if (lane >= o) { x.x += y; x.y += z; }
+            }
+            const int f = __ffs(__ballot_sync(0xffffffffu, x.x > u - front)) - 1;
+            front += __shfl_sync(0xffffffffu, x.x - c.x, f);
+            t += __shfl_sync(0xffffffffu, x.y - c.y, f);
+            w.seq = i0 + f;
+            t += w.seek(a, QB, u - front, gap);
+        }
         if (lane == 0) {
             run_ends[warp] = t;
             if (warp == 0) {
-                run = w;
-                // places of the segment's first tile and of the end of its last; cut for the first time?
-                const int from = u0 + gap - w.step, to = from + w.t.steps, s0 = w.q * QB;
-                const bool cut = w.step > 0 && from >= u0 - share;
-                static_cast<KpCut *>(a.plan)[blockIdx.x] = {cut ? (to - 1) / share - (int)blockIdx.x + 2 : 0, w.row0 + s0, min(QB, w.rows - s0) * group, w.head};
+                KpCut cut = {};
+                if (u < total) {
+                    run = w;
+                    // places of the segment's first tile and of the end of its last; cut for the first time?
+                    const int from = u + gap - w.step, to = from + w.t.steps, s0 = w.q * QB;
+                    if (w.step > 0 && from >= u - share) cut = {(to - 1) / share - (int)blockIdx.x + 2, w.row0 + s0, min(QB, w.rows - s0) * group, w.head};
+                }
+                static_cast<KpCut *>(a.plan)[blockIdx.x] = cut;
             }
         }
     }
-    if (tid == 0 && u0 >= u1) static_cast<KpCut *>(a.plan)[blockIdx.x].parts = 0;
     __syncthreads();
-    const int n = u0 < u1 ? run_ends[1] - run_ends[0] : 0;
+    const int n = run_ends[1] - run_ends[0];
     // TMEM columns: queries (both terms), scores and then weights [2] x 128, weighted values
     const uint32_t t_q = tmem, t_s = tmem + 128, t_o = tmem + 384;
     auto par = [](int i) { return (uint32_t)(i >> 1) & 1u; };
@@ -842,7 +836,7 @@ __global__ void __launch_bounds__(256) kv_prompt_merge_kernel(const __grid_const
 }
 
 // ---- host -----------------------------------------------------------------------------------------
-static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + (n_seq + 1) * sizeof(int2); }
+static size_t kp_smem(size_t d, size_t n_seq) { return (d == 64 ? KpGeom<64>::PLAN : KpGeom<128>::PLAN) + n_seq * sizeof(int2); }
 static size_t kp_plan_bytes(const yscv_cuda_ctx *ctx) { return (ctx->sm_count * sizeof(KpCut) + 31) & ~(size_t)31; }
 
 size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head) {
