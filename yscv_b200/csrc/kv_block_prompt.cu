@@ -19,11 +19,11 @@
 // maxima to each other, a tile takes 3950 cycles, with four warps on each of two tiles 3600.
 // Registers are moved between the warpgroups: 640 threads x 96 = 128 x (56 + 72 + 96 + 96 + 160).
 //
-// Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, with room for KP_BEGIN tiles in front of each
-// segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
+// Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, KP_TILE places each, with KP_BEGIN places in front of
+// each segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
 // kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and causal prompts, whose first
-// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 165 us; an earlier form with longer beginnings took
-// 456 us with tiles alone and 210 with room for two).
+// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 151 us; 162 with four places in front of a segment,
+// 154 with five).
 // Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128; what holds a tile for 3600
 // is the chain of its two products and its softmax, with as many tiles on their way as TMEM has room for (two), and the issue slots,
 // of which a tile takes 2100 of each scheduler.
@@ -36,7 +36,8 @@
 
 namespace yscv {
 
-constexpr int KP_KEYS = 128, KP_ROWS = 128, KP_THREADS = 640, KP_NOTES = 8, KP_BEGIN = 1;
+constexpr int KP_KEYS = 128, KP_ROWS = 128, KP_THREADS = 640, KP_NOTES = 8;
+constexpr int KP_TILE = 4, KP_BEGIN = 6;   // places that a tile takes, and the beginning and end of a segment
 
 template <int D> struct KpGeom {
     static constexpr int OPERAND = KP_KEYS * D * 2, RAW = KP_KEYS * D;   // keys, or values, of a tile, in fp16 and as cached
@@ -145,15 +146,15 @@ struct KpWalk {
         rows = r.rows;
         row0 = r.row0;
     }
-    // The first tile at place `left` of sequence `seq` or behind it (there is one), a warp together. Returns the tiles of the sequence in
-    // front of it; `gap`: places between the two.
-    __device__ int seek(const KvAttention &a, int QB, int left, int &gap) {
+    // The tile that place `left` of sequence `seq` is within, or whose beginning it is in front of, a warp together. Returns the tiles of
+    // the sequence in front of it; `in`: places of its segment in front of that place.
+    __device__ int seek(const KvAttention &a, int QB, int left, int &in) {
         load(a);
         int tiles = 0;
         const int lane = threadIdx.x & 31;
         for (int q0 = 0;; q0 += 32) {
             const int steps = q0 + lane < kp_tiles(rows, QB) ? kp_tile(a, start, rows, QB, q0 + lane).steps : 0;
-            const int n = steps > 0 ? (steps + KP_BEGIN) * a.l.n_kv : 0;
+            const int n = steps > 0 ? (KP_TILE * steps + KP_BEGIN) * a.l.n_kv : 0;
             int upto = n, tiles_upto = steps * a.l.n_kv;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -172,10 +173,10 @@ struct KpWalk {
             tiles += __shfl_sync(0xffffffffu, tiles_upto, 31);
         }
         t = kp_tile(a, start, rows, QB, q);
-        head = left / (t.steps + KP_BEGIN);
-        const int in = left - head * (t.steps + KP_BEGIN);
-        gap = max(0, KP_BEGIN - in);
-        step = max(0, in - KP_BEGIN);
+        const int places = KP_TILE * t.steps + KP_BEGIN;
+        head = left / places;
+        in = left - head * places;
+        step = max(0, in - KP_BEGIN) / KP_TILE;
         return tiles + head * t.steps + step;
     }
     // the first step of the next segment (there is one)
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
         const KvSeqRows r = kv_rows(a, i);
         const int n = kp_steps(a, r.start, r.rows, QB);
         if (lane == 0) {
-            counted[i] = make_int2((n + KP_BEGIN * kp_tiles(r.rows, QB)) * a.l.n_kv, n * a.l.n_kv);
+            counted[i] = make_int2((KP_TILE * n + KP_BEGIN * kp_tiles(r.rows, QB)) * a.l.n_kv, n * a.l.n_kv);
             if (blockIdx.x == 0) kv_rows_status(a, r);
         }
     }
@@ -280,10 +281,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             total += __reduce_add_sync(0xffffffffu, c.x);
             t += __reduce_add_sync(0xffffffffu, c.y);
         }
-        const int share = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x), u0 = (int)min((long long)total, (long long)blockIdx.x * share);
+        // (no run in the middle of a segment is without a tile)
+        const int share = max((int)(((unsigned)total + gridDim.x - 1) / gridDim.x), KP_TILE), u0 = (int)min((long long)total, (long long)blockIdx.x * share);
         const int u = warp == 0 ? u0 : (int)min((long long)total, (long long)u0 + share);
         KpWalk w;
-        int gap = 0;
+        int in = 0;
         if (u < total) {
             int i0 = 0, front = 0;
             t = 0;
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             front += __shfl_sync(0xffffffffu, x.x - c.x, f);
             t += __shfl_sync(0xffffffffu, x.y - c.y, f);
             w.seq = i0 + f;
-            t += w.seek(a, QB, u - front, gap);
+            t += w.seek(a, QB, u - front, in);
         }
         if (lane == 0) {
             run_ends[warp] = t;
@@ -310,9 +312,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 KpCut cut = {};
                 if (u < total) {
                     run = w;
-                    // places of the segment's first tile and of the end of its last; cut for the first time?
-                    const int from = u + gap - w.step, to = from + w.t.steps, s0 = w.q * QB;
-                    if (w.step > 0 && from >= u - share) cut = {(to - 1) / share - (int)blockIdx.x + 2, w.row0 + s0, min(QB, w.rows - s0) * group, w.head};
+                    // a tile is in the run of its last place; is the segment cut for the first time?
+                    const int first = u - in + KP_BEGIN + KP_TILE - 1, last = first + KP_TILE * (w.t.steps - 1), s0 = w.q * QB;
+                    if (w.step > 0 && first / share == (int)blockIdx.x - 1)
+                        cut = {last / share - (int)blockIdx.x + 2, w.row0 + s0, min(QB, w.rows - s0) * group, w.head};
                 }
                 static_cast<KpCut *>(a.plan)[blockIdx.x] = cut;
             }
@@ -852,7 +855,7 @@ size_t kv_prompt_bytes(const yscv_cuda_ctx *ctx, size_t d_head) {
 bool kv_prompt_takes(const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows) {
     if ((pool->d_head != 64 && pool->d_head != 128) || group > KP_ROWS || kp_smem(pool->d_head, pool->n_seq) > 226 * 1024) return false;
     // (places are counted in 32 bits)
-    const size_t tiles = rows / (KP_ROWS / group) + pool->n_seq, steps = pool->max_pages * pool->page / KP_KEYS + 2 + KP_BEGIN;
+    const size_t tiles = rows / (KP_ROWS / group) + pool->n_seq, steps = KP_TILE * (pool->max_pages * pool->page / KP_KEYS + 2) + KP_BEGIN;
     if (tiles >= (1u << 31) / pool->n_kv / steps) return false;
     return most_rows * group > 32;
 }
