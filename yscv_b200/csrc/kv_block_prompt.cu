@@ -697,7 +697,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 if (g + 2 < groups) kp_ld16(s_at + 16 * g + 32, v);
                 weights(g + 1, u, k2.y, l2.y, i2.y);
             }
-            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             if (groups == 0) kp_wait_ld16(v);
 #pragma unroll 1
             for (int g = groups; g < 8; g += 2) {
@@ -706,6 +705,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 kp_st16(s_at + 16 * g, none);
                 kp_st16(s_at + 16 * g + 16, none);
             }
+            asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             stats[(i & 3) * KP_ROWS + row] = make_float2(mx, sum);
             at_fence_before();
             __syncwarp();
