@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
         next_id = -1;
         if (lane < groups_of(f)) {
             const int at = (f.s.lo + f.step * KA_STEP + KV_GROUP * lane) >> a.l.page_shift;
-            if (at < a.l.max_pages) next_id = __ldg(a.l.table + (size_t)f.seq * a.l.max_pages + at);
+            if (at < a.l.max_pages) next_id = a.l.table[(size_t)f.seq * a.l.max_pages + at];
             if (at >= a.l.max_pages) atomicExch(a.status, YSCV_DEV_POS_OVERFLOW);
             else if (next_id < 0 || next_id >= a.l.n_pages) { next_id = -1; atomicExch(a.status, YSCV_DEV_BAD_NUMBER); }
         }
@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
         next_vs = -1.0f;
         if (there) {
             const size_t s_at = (size_t)next_id * a.l.n_kv + f.head;
-            next_ks = __ldg(a.l.ks + s_at);
-            next_vs = __ldg(a.l.vs + s_at);
+            next_ks = a.l.ks[s_at];
+            next_vs = a.l.vs[s_at];
             from = kv_group_at(a.l, next_id, f.head, ((f.s.lo + f.step * KA_STEP + KV_GROUP * lane) & (a.l.page - 1)) / KV_GROUP);
             if (lane % piece == 0) bytes = min(piece, groups_of(f) - lane) * (KV_GROUP * D);
         }
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
                 auto load = [&](int k, int h) {
                     const float *p = src + 32 * k + 16 * h + 4 * t;
                     if (!live) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    return a.wide ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+                    return a.wide ? *reinterpret_cast<const float4 *>(p) : make_float4(p[0], p[1], p[2], p[3]);
                 };
                 float most = 0.0f, bad = 0.0f;
 #pragma unroll 4

@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                         const float *from = a.q + (size_t)(w.row0 + s0 + r / group) * a.q_stride + (size_t)(w.head * group + r % group) * D;
                         unsigned char *to = smem + G::Q_AT + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) *reinterpret_cast<float *>(to + c * G::Q_PART) = __ldg(from + 32 * c + lane);
+                        for (int c = 0; c < D / 32; ++c) *reinterpret_cast<float *>(to + c * G::Q_PART) = from[32 * c + lane];
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(qstaged);
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 const int key = w.t.lo + w.step * KP_KEYS + KV_GROUP * lane, at = key >> a.l.page_shift;
                 id = -1;
                 if (lane < 8 && key < w.t.hi) {
-                    if (at < a.l.max_pages) id = __ldg(a.l.table + (size_t)w.seq * a.l.max_pages + at);
+                    if (at < a.l.max_pages) id = a.l.table[(size_t)w.seq * a.l.max_pages + at];
                     else atomicExch(a.status, YSCV_DEV_POS_OVERFLOW);
                 }
             };
@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 if (wanted && !there && (key >> a.l.page_shift) < a.l.max_pages) atomicExch(a.status, YSCV_DEV_BAD_NUMBER);
                 float ks = 1.0f, vs = -1.0f;
                 if (!values && there) {
-                    ks = __ldg(a.l.ks + (size_t)id * a.l.n_kv + w.head);
-                    vs = __ldg(a.l.vs + (size_t)id * a.l.n_kv + w.head);
+                    ks = a.l.ks[(size_t)id * a.l.n_kv + w.head];
+                    vs = a.l.vs[(size_t)id * a.l.n_kv + w.head];
                 }
                 const int group_in = (key & (a.l.page - 1)) / KV_GROUP;
                 const unsigned groups = __ballot_sync(0xffffffffu, there);
