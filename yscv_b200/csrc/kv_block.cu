@@ -248,8 +248,19 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
     }
 }
 
-// Cached rows as f32: a CTA per (page, head, keys or values), a warp per group of 16 tokens. Keys: a lane has four d of a token, so
-// that a row leaves in whole lines; values: one d of 16 tokens.
+// four numbers times s: 2^23 + q + 128, less that (a conversion is a quarter of the rate)
+__device__ __forceinline__ float4 kv_floats(uint32_t w, float s) {
+    const uint32_t x = w ^ 0x80808080u, top = 0x4B000000u;
+    auto number = [&](int sel) { return __uint_as_float(__byte_perm(x, top, sel)); };
+    const uint64_t off = f2(-8388736.0f, -8388736.0f), by = f2(s, s);
+    float4 y;
+    f2_get(f2_mul(f2_add(f2(number(0x7440), number(0x7441)), off), by), y.x, y.y);
+    f2_get(f2_mul(f2_add(f2(number(0x7442), number(0x7443)), off), by), y.z, y.w);
+    return y;
+}
+
+// Cached rows as f32: a CTA per (page, head, keys or values), a warp per group of 16 tokens. A lane has four d, keys as they lie,
+// values turned around, so that a row leaves in whole lines. 3700 rows of 8 heads of 128: 13.3 us with a d of 16 tokens per lane, 10.1 so.
 __global__ void __launch_bounds__(128, 8) kv_read_kernel(const KvLayer l, const KvRows rows, int per_seq, float *__restrict__ k_out, float *__restrict__ v_out,
                                                       int wide, int *__restrict__ status) {
     pdl_wait();
@@ -279,14 +290,30 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const KvLayer l, const 
             const int a = max(t0, g * KV_GROUP), b = min(t1, g * KV_GROUP + KV_GROUP);
             const int8_t *group = page + (size_t)g * (KV_GROUP * l.d);
             float *o = out + (size_t)a * rows.stride;
+            auto put = [&](float *p, uint32_t w) {
+                const float4 y = kv_floats(w, s);
+                if (wide) {
+                    *reinterpret_cast<float4 *>(p) = y;
+                } else {
+                    p[0] = y.x; p[1] = y.y; p[2] = y.z; p[3] = y.w;
+                }
+            };
             if (values) {
-                for (int c = lane; c < l.d; c += 32) {
-                    const uint4 w = reinterpret_cast<const uint4 *>(group)[c];
-                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                for (int c = lane; c < l.d >> 2; c += 32) {
+                    uint4 w[4];
 #pragma unroll
-                    for (int j = 0; j < KV_GROUP; ++j) {
-                        const int t = g * KV_GROUP + j;
-                        if (t >= a && t < b) o[(size_t)(t - a) * rows.stride + c] = (float)(int8_t)(word[j >> 2] >> (8 * (j & 3))) * s;
+                    for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint4 *>(group)[4 * c + j];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        auto word = [&](const uint4 &y) { return q == 0 ? y.x : q == 1 ? y.y : q == 2 ? y.z : y.w; };
+                        const uint32_t in[4] = {word(w[0]), word(w[1]), word(w[2]), word(w[3])};
+                        uint32_t out[4];
+                        kv_turn(in, out);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int t = g * KV_GROUP + 4 * q + j;
+                            if (t >= a && t < b) put(o + (size_t)(t - a) * rows.stride + 4 * c, out[j]);
+                        }
                     }
                 }
             } else {
@@ -294,14 +321,7 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const KvLayer l, const 
                     const int8_t *from = group + (c >> 2) * 256 + (c & 3) * 4 + (a - g * KV_GROUP) * 16;
 #pragma unroll 8
                     for (int t = 0; t < b - a; ++t) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t *>(from + t * 16);
-                        const float4 y = make_float4((float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s, (float)(int8_t)(w >> 16) * s, (float)(int8_t)(w >> 24) * s);
-                        float *p = o + (size_t)t * rows.stride + 4 * c;
-                        if (wide) {
-                            *reinterpret_cast<float4 *>(p) = y;
-                        } else {
-                            p[0] = y.x; p[1] = y.y; p[2] = y.z; p[3] = y.w;
-                        }
+                        put(o + (size_t)t * rows.stride + 4 * c, *reinterpret_cast<const uint32_t *>(from + t * 16));
                     }
                 }
             }
