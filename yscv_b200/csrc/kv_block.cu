@@ -11,6 +11,7 @@
 // share: byte by byte). 3700 rows of 8 heads of 128, pages of 32: 33.9 us with keys stored 4 bytes and value rows gathered a
 // byte at a time and an index division per access, 18.5 us, 16.5 with four numbers rounded at once (kv_round4).
 #include <cfloat>
+#include <type_traits>
 
 #include "attention_tc.cuh"
 #include "kv_pool.cuh"
@@ -127,7 +128,8 @@ __device__ __forceinline__ void kv_turn(const uint32_t (&w)[4], uint32_t (&out)[
     out[3] = __byte_perm(c, d, 0x7632);
 }
 
-template <int T>
+// (D: the head size, 0 for any; a division by it is a shift where it is known)
+template <int T, int D>
 __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l, const float *__restrict__ k, const float *__restrict__ v, const KvRows rows,
                                                       int per_seq, int wide, int *__restrict__ status) {
     extern __shared__ __align__(16) unsigned char stage[];   // [tokens][kv_stage_pitch(d)]
@@ -140,8 +142,8 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
     if (!sp.live) return;
     const long long end = (long long)sp.p0 + sp.rows;
     // a thread has four d of every `step`-th token
-    const int d4 = l.d >> 2, step = T / d4, c = tid % d4, first = tid / d4 < step ? tid / d4 : 1 << 30, pitch = kv_stage_pitch(l.d);
-    const float *src = (values ? v : k) + (size_t)sp.row0 * rows.stride + (size_t)head * l.d + 4 * c;
+    const int d = D ? D : l.d, d4 = d >> 2, step = T / d4, c = tid % d4, first = tid / d4 < step ? tid / d4 : 1 << 30, pitch = kv_stage_pitch(d);
+    const float *src = (values ? v : k) + (size_t)sp.row0 * rows.stride + (size_t)head * d + 4 * c;
     for (long long pg = (sp.p0 >> l.page_shift) + blockIdx.x % per_seq; (pg << l.page_shift) < end; pg += per_seq) {
         if (pg >= l.max_pages) {
             if (tid == 0) atomicExch(status, YSCV_DEV_POS_OVERFLOW);
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
             // what the page holds, once more: rows of 16 bytes, one token's keys or 16 tokens' values
             const float ratio = __fdiv_rn(s_old, s);
             const int groups = (t0 + KV_GROUP - 1) / KV_GROUP;
-            for (int i = tid; i < groups * l.d; i += T) {
-                const int in = i % l.d, token = (i / l.d) * KV_GROUP + (values ? 0 : in % KV_GROUP);
+            for (int i = tid; i < groups * d; i += T) {
+                const int in = i % d, token = (i / d) * KV_GROUP + (values ? 0 : in % KV_GROUP);
                 if (token >= t0) continue;
                 uint4 *p = reinterpret_cast<uint4 *>(page) + i;
                 uint4 w = *p;
@@ -211,9 +213,9 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
         for (int t = first + step * KVB_KEEP; t < n; t += step) put(t, kv_load4(row + (size_t)t * rows.stride, wide));
         __syncthreads();   // (the last value row's bytes of new tokens follow those that were rounded again)
         if (!values) {
-            const int i1 = ((t1 + KV_GROUP - 1) / KV_GROUP) * l.d;
-            for (int i = t0 / KV_GROUP * l.d + tid; i < i1; i += T) {
-                const int g = i / l.d, in = i - g * l.d, t = g * KV_GROUP + in % KV_GROUP - t0;
+            const int i1 = ((t1 + KV_GROUP - 1) / KV_GROUP) * d;
+            for (int i = t0 / KV_GROUP * d + tid; i < i1; i += T) {
+                const int g = i / d, in = i - g * d, t = g * KV_GROUP + in % KV_GROUP - t0;
                 if (t >= 0 && t < n) reinterpret_cast<uint4 *>(page)[i] = *reinterpret_cast<const uint4 *>(stage + t * pitch + (in / KV_GROUP) * 16);
             }
         } else {
@@ -369,7 +371,14 @@ int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
     const KvRows rows = {d_offsets, d_start, row_stride};
     // (room for a whole page: a sequence may have more rows than were expected)
     const size_t smem = (size_t)l.page * kv_stage_pitch(l.d);
-    auto kern = threads == 64 ? kv_append_kernel<64> : threads == 128 ? kv_append_kernel<128> : threads == 256 ? kv_append_kernel<256> : kv_append_kernel<512>;
+    auto of = [&](auto size) {
+        constexpr int D = decltype(size)::value;
+        return threads == 64 ? kv_append_kernel<64, D> : threads == 128 ? kv_append_kernel<128, D> : threads == 256 ? kv_append_kernel<256, D> : kv_append_kernel<512, D>;
+    };
+    auto kern = l.d == 64    ? of(std::integral_constant<int, 64>())
+                : l.d == 128 ? of(std::integral_constant<int, 128>())
+                : l.d == 256 ? of(std::integral_constant<int, 256>())
+                             : of(std::integral_constant<int, 0>());
     YSCV_CUDA_TRY(launch_pdl(kern, grid, dim3((unsigned)threads), smem, ctx->stream, l, d_k, d_v, rows, per, (int)wide, ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
     ctx->launches++;
