@@ -492,7 +492,8 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
 // Adds the records of a segment that several warps shared: for each (sequence, KV head) W warps a pair, P pairs a CTA. Either one warp a
 // pair, or, where there are fewer (sequence, head, pair)s than four an SM, sixteen, a share of the records each (one sequence of
 // 131000 keys, 64 / 8 heads: 8 warps 69.7 us for both kernels, 16 65.9, 32 64.5, but 10.1 us for one of 200 keys where 16 take 9.6).
-// 64 sequences, four warps a pair for all: 122 us, one warp 117.5.
+// 64 sequences, four warps a pair for all: 122 us, one warp 117.5. A table of 2048 positions has 33 records at most, which a warp adds by
+// itself (one sequence of 200 keys: 9.3 us, 9.5 with sixteen).
 template <int D, int R, int W, int P>
 __global__ void __launch_bounds__(32 * W * P) kv_attention_merge_kernel(const __grid_constant__ KvAttention a) {
     static_assert(W == 1 || P == 1, "the shares of a pair are added by its whole CTA");
@@ -616,7 +617,7 @@ template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttenti
     YSCV_CUDA_TRY(launch_pdl(kern, dim3((unsigned)ctx->sm_count), dim3(KaGeom<D, R>::WARPS * 32), ka_smem(D, R, a.l.n_seq), ctx->stream, a));
     ctx->launches++;
     const size_t z = pairs < 1024 ? pairs : 1024;
-    const bool few = (size_t)a.l.n_seq * a.l.n_kv * z < (size_t)4 * ctx->sm_count;
+    const bool few = (size_t)a.l.n_seq * a.l.n_kv * z < (size_t)4 * ctx->sm_count && a.room > 32 * KA_STEP;
     YSCV_CUDA_TRY(launch_pdl(few ? kv_attention_merge_kernel<D, R, 16, 1> : kv_attention_merge_kernel<D, R, 1, 8>,
                              dim3((unsigned)a.l.n_seq, (unsigned)a.l.n_kv, (unsigned)(few ? z : (z + 7) / 8)), dim3(few ? 512 : 256), 0, ctx->stream, a));
     ctx->launches++;
