@@ -675,6 +675,36 @@ def test_attention_of_longer_rows(d, page, counts, start):
     ctx.close()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_of_as_many_sequences_as_there_may_be(d):
+    """The largest n_seq that is not refused, of which the first, the last and one between take part."""
+    ctx = _context()
+
+    def takes(n):
+        pool = Pool(ctx, n_pages=2, n_kv=1, d=d, page=16, n_seq=1, max_pages=4)
+        try:
+            ctx.kv_block_attention_workspace(pool.handle(n_seq=n), 2, 8, 1)
+        except yscv_b200.YscvCudaError:
+            return False
+        return True
+
+    lo, hi = 1, 1 << 17
+    while hi - lo > 1:
+        lo, hi = ((lo + hi) // 2, hi) if takes((lo + hi) // 2) else (lo, (lo + hi) // 2)
+    assert lo > 1000
+    pool = Pool(ctx, n_pages=20, n_kv=1, d=d, page=16, n_seq=lo, max_pages=4)
+    counts, start = [0] * lo, [-1] * lo
+    for i, m, s in ((0, 3, 20), (lo // 2, 1, 63), (lo - 1, 4, 0)):
+        counts[i], start[i] = m, s
+    pool.give([max(0, s) + m if m else 0 for s, m in zip(start, counts)])
+    q = torch.randn(8, 2, d, device="cuda", generator=pool.g)
+    for most in (1, 100):
+        got, live = _attend(ctx, pool, q, counts, start, most=most)
+        _done(ctx)
+        _check(got, live, *attention(pool, q, start, counts))
+    ctx.close()
+
+
 @pytest.mark.parametrize("most", [1, 70])
 def test_attention_of_pages_whose_scales_are_zero(most):
     """Keys of 0 take part with a score of 0, values of 0 with their weight: beside others, and alone."""

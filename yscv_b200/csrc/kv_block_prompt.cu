@@ -47,7 +47,7 @@ template <int D> struct KpGeom {
     static constexpr int Q_PART = KP_ROWS * 128;
     static constexpr int STATS = Q_AT + D / 32 * Q_PART;               // [4][128] {maximum, sum} of a tile's rows
     static constexpr int NOTES = STATS + 4096;
-    static constexpr int SCALES = NOTES + KP_NOTES * 128;      // [4][128] powers of two that the queries of a segment were multiplied by (read until its last tile)
+    static constexpr int SCALES = NOTES + KP_NOTES * 128;      // [4][128] powers of two of a segment's queries, read until its last tile
     static constexpr int BARS = SCALES + 4 * KP_ROWS * 4;
     static constexpr int PLAN = BARS + 256;
 };
@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     __shared__ int heads[KP_NOTES], begun[KP_NOTES], segments[KP_NOTES];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = smem_u32(smem), bars = base + G::BARS;
-    // [2] by tile & 1, each used again two tiles later (pfull: another two for the tile's second 64 keys); nfull [KP_NOTES]; from kfull on one phase a tile; from qstaged on one a segment
+    // [2] by tile & 1, each used again two tiles later (pfull: another two for the tile's second 64 keys); nfull [KP_NOTES]; from kfull on
+    // one phase a tile; from qstaged on one a segment
     const uint32_t vfull = bars, sfull = bars + 16, pfull = bars + 32, ofull = bars + 64, ofree = bars + 80;
     const uint32_t nfull = bars + 96, kfull = bars + 160, raw_k = bars + 176, raw_v = bars + 184, raw_k_free = bars + 192;
     const uint32_t raw_v_free = bars + 200, qstaged = bars + 216, qtaken = bars + 224, qfull = bars + 232;
