@@ -13,7 +13,7 @@
 //   warps 4-7    the tile's bytes as fp16 operands
 //   warps 8-15   softmax, a thread a row, two tiles at a time: the queries' two terms to TMEM for a segment's first tile; scores from
 //                TMEM, the tile's own maximum and sum, weights back to where the scores were. They keep nothing from tile to tile
-//   warps 16-19  the output in registers, a thread per row: o = o 2^(M - M') + O 2^(m - M'), and results
+//   warps 16-19  the output in registers, a thread per row: o = o + O 2^(m - M), M at most 2^8 below the running maximum, and results
 // With the output in the softmax threads' registers those have too few left to keep several exponentials in flight: 2048 x 2048
 // keys, 64 / 8 heads of 128, 507 us, a tile of 128 rows 6300 cycles. With all eight softmax warps on one tile, which then hand its
 // maxima to each other, a tile takes 3950 cycles, with four warps on each of two tiles 3600.
@@ -22,8 +22,8 @@
 // Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, KP_TILE places each, with KP_BEGIN places in front of
 // each segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
 // kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and causal prompts, whose first
-// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 151 us; 162 with four places in front of a segment,
-// 154 with five).
+// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 151 us where it took 162 with four
+// places in front of a segment, 154 with five; 146 now).
 // Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128; what holds a tile for 3600
 // is the chain of its two products and its softmax, with as many tiles on their way as TMEM has room for (two), and the issue slots,
 // of which a tile takes 2100 of each scheduler.
@@ -726,8 +726,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             alive = __all_sync(0xffffffffu, kp_wait(ofull + st * 8, par(i)));
             if (!alive) break;
             at_fence_after();
-            float t0[16], t1[16];
-            kp_ld16(o_at, t0);
             const KpNote &note = notes[i % KP_NOTES];
             const float2 ms = stats[(i & 3) * KP_ROWS + row];
             if (note.begins) {
@@ -737,23 +735,33 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < D / 2; ++j) o[j] = 0ull;
             }
-            const float m_new = fmaxf(m, ms.x);
-            const float alpha = m_new == -INFINITY ? 1.0f : at_exp2(m - m_new), beta = m_new == -INFINITY ? 0.0f : at_exp2(ms.x - m_new);
-            l = fmaf(l, alpha, beta * ms.y);
-            m = m_new;
+            // What the output is relative to follows the maximum only where that is 2^8 above it, which after a segment's first tiles is
+            // rare (pieces of three prompts: 88 us, 91 with a factor on the output for every tile)
+            if (__any_sync(0xffffffffu, ms.x > m + 8.0f)) {
+                const float m_new = fmaxf(m, ms.x), alpha = m_new == -INFINITY ? 1.0f : at_exp2(m - m_new);
+                const uint64_t al2 = f2(alpha, alpha);
+                l *= alpha;
+                m = m_new;
+#pragma unroll
+                for (int j = 0; j < D / 2; ++j) o[j] = f2_mul(o[j], al2);
+            }
+            float t0[16], t1[16];
+            kp_ld16(o_at, t0);
+            const float beta = m == -INFINITY ? 0.0f : at_exp2(ms.x - m);
+            l = fmaf(beta, ms.y, l);
             const float b = beta * fmaxf(note.vmost, 0.0f);
-            const uint64_t al2 = f2(alpha, alpha), b2 = f2(b, b);
+            const uint64_t b2 = f2(b, b);
             // (read as fast as it goes: the next product with weights waits for it)
 #pragma unroll
             for (int j0 = 0; j0 < D; j0 += 32) {
                 kp_wait_ld16(t0);
                 kp_ld16(o_at + j0 + 16, t1);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[j0 / 2 + e] = f2_fma(o[j0 / 2 + e], al2, f2_mul(f2(t0[2 * e], t0[2 * e + 1]), b2));
+                for (int e = 0; e < 8; ++e) o[j0 / 2 + e] = f2_fma(f2(t0[2 * e], t0[2 * e + 1]), b2, o[j0 / 2 + e]);
                 kp_wait_ld16(t1);
                 if (j0 + 32 < D) kp_ld16(o_at + j0 + 32, t0);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[j0 / 2 + 8 + e] = f2_fma(o[j0 / 2 + 8 + e], al2, f2_mul(f2(t1[2 * e], t1[2 * e + 1]), b2));
+                for (int e = 0; e < 8; ++e) o[j0 / 2 + 8 + e] = f2_fma(f2(t1[2 * e], t1[2 * e + 1]), b2, o[j0 / 2 + 8 + e]);
             }
             at_fence_before();
             __syncwarp();
