@@ -675,6 +675,25 @@ def test_attention_of_longer_rows(d, page, counts, start):
     ctx.close()
 
 
+def test_attention_of_sequences_that_overlap_without_end():
+    """Falling offsets can let sequences claim the same rows, so many times that their work is beyond counting: told, and left alone."""
+    ctx = _context()
+    rows, n_seq = 4096, 80
+    pool = Pool(ctx, n_pages=2, n_kv=1, d=64, page=128, n_seq=n_seq, max_pages=8192)
+    q = torch.zeros(rows, 128, 64, device="cuda")
+    out = torch.full_like(q, 3.0)
+    off, start = i32([rows * (i % 2) for i in range(n_seq + 1)]), i32([8192 * 128 - rows] * n_seq)
+    handle = pool.handle()
+    ws = torch.empty(ctx.kv_block_attention_workspace(handle, 128, rows, 100), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ctx.kv_block_attention_dev(handle, 0, q.data_ptr(), 128 * 64, 128, off.data_ptr(), start.data_ptr(), rows, 100, True, 0, 0.0, out.data_ptr(), 128 * 64,
+                               ws.data_ptr(), ws.numel())
+    assert "tcgen05" in ctx.last_kernel()
+    _done(ctx, 4)
+    assert torch.all(out == 3.0)
+    ctx.close()
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attention_of_as_many_sequences_as_there_may_be(d):
     """The largest n_seq that is not refused, of which the first, the last and one between take part."""

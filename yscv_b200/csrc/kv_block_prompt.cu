@@ -276,11 +276,18 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
     if (warp < 2) {                         // where this run begins, and where the next does
         const int n_seq = a.l.n_seq;
         auto counts = [&](int i0) { return i0 + lane < n_seq ? counted[i0 + lane] : make_int2(0, 0); };
-        int total = 0, t = 0;               // places of the call; tiles in front of place u
+        long long places = 0;               // of the call
+        int t = 0;                          // tiles in front of place u
         for (int i0 = 0; i0 < n_seq; i0 += 32) {
             const int2 c = counts(i0);
-            total += __reduce_add_sync(0xffffffffu, c.x);
+            places += ((long long)__reduce_add_sync(0xffffffffu, c.x >> 16) << 16) + __reduce_add_sync(0xffffffffu, c.x & 0xffff);
             t += __reduce_add_sync(0xffffffffu, c.y);
+        }
+        // (more than 32 bits hold: only of sequences that overlap. Then nobody takes part.)
+        const int total = places <= INT_MAX ? (int)places : 0;
+        if (places > INT_MAX) {
+            t = 0;
+            if (blockIdx.x == 0 && tid == 0) atomicExch(a.status, YSCV_DEV_BAD_NUMBER);
         }
         // (no run in the middle of a segment is without a tile)
         const int share = max((int)(((unsigned)total + gridDim.x - 1) / gridDim.x), KP_TILE), u0 = (int)min((long long)total, (long long)blockIdx.x * share);
