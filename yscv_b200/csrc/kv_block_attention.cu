@@ -631,6 +631,9 @@ static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool 
                                                                        : ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * group));
 }
 
+// A guess of no rows may be wrong: what a call launches and what it needs both go by one row at least
+static size_t ka_guess(size_t most_rows) { return most_rows > 0 ? most_rows : 1; }
+
 static int ka_check(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows, size_t most_rows) {
     if (!ctx) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null");
     if (const int rc = kv_check_pool(pool)) return rc;
@@ -654,7 +657,7 @@ int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_k
                                            size_t *bytes) {
     if (const int rc = ka_check(ctx, pool, n_q, rows, most_rows)) return rc;
     if (!bytes) return fail(YSCV_CUDA_ERR_BAD_ARG, "bytes is null");
-    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, rows, most_rows);
+    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, rows, ka_guess(most_rows));
     return YSCV_CUDA_OK;
 }
 
@@ -671,7 +674,8 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     if (d_q == d_out) return fail(YSCV_CUDA_ERR_BAD_ARG, "d_out is d_q");
     if (!(scale >= 0.0f && scale <= FLT_MAX)) return fail(YSCV_CUDA_ERR_BAD_ARG, "scale must be 0 (the default) or positive");
     if (reinterpret_cast<uintptr_t>(d_workspace) & 15) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "the workspace must be 16-byte aligned");
-    const size_t group = n_q / pool->n_kv, pairs = std::max(most_rows, (size_t)1) * group;   // (a guess of none may be wrong)
+    most_rows = ka_guess(most_rows);
+    const size_t group = n_q / pool->n_kv, pairs = most_rows * group;
     const int R = ka_rows(pool->d_head, pairs);
     const size_t need = attention_bytes(ctx, pool, group, rows, most_rows);
     if (workspace_bytes < need) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
