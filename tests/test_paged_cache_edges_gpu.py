@@ -1,11 +1,10 @@
 """The paged 8-bit KV cache where its calls are easily wrong: guesses of no rows, workspaces that serve several calls, pages without a
 scale or with very unlike ones, wrong offsets. Against float64 definitions (paged_pool.py)."""
-
 import pytest
 import torch
 
 from paged_pool import Pool, attention
-from test_paged_cache_gpu import _attend, _check, _context, _done
+from test_paged_cache_gpu import _append, _attend, _check, _context, _done
 
 pytestmark = pytest.mark.gpu
 
@@ -36,4 +35,41 @@ def test_attention_with_a_guess_of_no_rows_keeps_to_its_workspace(d, keys):
     _done(ctx)
     _check(got, live, *attention(pool, q, start, counts))
     assert torch.equal(ws[need[0]:], guard)
+    ctx.close()
+
+
+@pytest.mark.parametrize("most", [2, 80])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 37), (False, 20)])
+def test_attention_across_pages_whose_key_scales_are_zero(most, causal, window):
+    """Such a page's keys count with a score of 0 where a row sees them and not at all where it does not: a diagonal, a window's
+    border and a last page that is not full run through them."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=60, n_kv=2, d=64, page=16, n_seq=2, max_pages=30)
+    start, counts = [0, 130], [150, 70]
+    pool.give([150, 200])
+    for i in range(2):
+        pool.ks[:, pool.table[i, [0, 3, 4, 8, 9, 12]].clamp(min=0).long()] = 0.0
+    q = torch.randn(220, 8, 64, device="cuda", generator=pool.g)
+    got, live = _attend(ctx, pool, q, counts, start, causal, window, most=most)
+    assert ("tcgen05" in ctx.last_kernel()) == (most == 80)
+    _done(ctx)
+    _check(got, live, *attention(pool, q, start, counts, causal, window))
+    ctx.close()
+
+
+@pytest.mark.parametrize("most", [2, 80])
+@pytest.mark.parametrize("size,scale", [(1e-9, 0.0), (1e-30, 0.0), (1.0, 1e-42)])
+def test_attention_of_zero_keys_as_append_holds_them(most, size, scale):
+    """Small queries, or a small scale, over keys of 0 and others: scores below what fp32 holds are 0, what is hidden stays hidden."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=30, n_kv=1, d=128, page=32, n_seq=1, max_pages=10)
+    pool.give([200])
+    k, v = (torch.randn(200, 1, 128, device="cuda", generator=pool.g) for _ in range(2))
+    k[:90] = 0.0
+    k[170:] = 0.0
+    _append(ctx, pool, k, v, [200], [0])
+    q = torch.randn(200, 4, 128, device="cuda", generator=pool.g) * size
+    got, live = _attend(ctx, pool, q, [200], [0], scale=scale, most=most)
+    _done(ctx)
+    _check(got, live, *attention(pool, q, [0], [200], scale=scale))
     ctx.close()

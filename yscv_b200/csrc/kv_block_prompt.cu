@@ -640,6 +640,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             }
+            // (never 0, where pages have no scale or products leave fp32's range: a hidden key's -inf has to stay one. What a seen key's
+            // score, at most 2^29 here, becomes by it is 2^-97 at most, a weight's exponent of nothing)
+            auto times = [&](float k) { return fmaxf(to_log2 * k, FLT_MIN); };
             float mx = -INFINITY, v[16], u[16];
             kp_ld16(s_at, v);
 #pragma unroll 1
@@ -652,7 +655,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                         x = fmaxf(x, fmaxf(z[e], z[e + 1]));
                         y = fmaxf(y, fmaxf(z[e + 2], z[e + 3]));
                     }
-                    mx = fmaxf(mx, fmaxf(x, y) * (to_log2 * k));
+                    mx = fmaxf(mx, fmaxf(x, y) * times(k));
                 };
                 kp_wait_ld16(v);
                 kp_ld16(s_at + 16 * g + 16, u);
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 if (lane == 0) mbar_arrive(pfull + st * 8);
             };
             auto weights = [&](int g, const float (&v)[16], float k, float lv, float inv) {
-                const float c = to_log2 * k, og = off + lv;
+                const float c = times(k), og = off + lv;
                 const uint64_t c2 = f2(c, c), og2 = f2(og, og), minus = f2(-1.0f, -1.0f);
                 uint32_t p[16];               // leading terms of 16 weights, remainders
                 uint64_t s2 = 0ull;
