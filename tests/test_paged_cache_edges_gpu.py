@@ -1,5 +1,7 @@
 """The paged 8-bit KV cache where its calls are easily wrong: guesses of no rows, workspaces that serve several calls, pages without a
 scale or with very unlike ones, wrong offsets. Against float64 definitions (paged_pool.py)."""
+import math
+
 import pytest
 import torch
 
@@ -72,4 +74,52 @@ def test_attention_of_zero_keys_as_append_holds_them(most, size, scale):
     got, live = _attend(ctx, pool, q, [200], [0], scale=scale, most=most)
     _done(ctx)
     _check(got, live, *attention(pool, q, [0], [200], scale=scale))
+    ctx.close()
+
+
+def _by_what_a_row_sees(pool, q, start, counts, causal, window):
+    """float64 result, and a bound that goes by the values a row sees: A, its weighted mean of |scale| * 127, and not by the largest
+    value of all. As in paged_pool.attention() a weight is off relatively by its score's error (twice) and 2^-21; what is less is the error
+    of a weight that is rounded to whole numbers: half a unit, of which the largest weight times scale of a row's 64 keys has 2^22 at least,
+    so that 64 of them are off by 64 * 2^-23 A. Two fp16 terms (the other kernel) are off by less. Sums over steps as there."""
+    n_q, d, n_kv = q.shape[1], q.shape[2], pool.n_kv
+    out, tol, row = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda"), 0
+    for i, (s0, m) in enumerate(zip(start, counts)):
+        k, v = pool.rows(i, s0 + m)
+        here, key = torch.arange(s0, s0 + m, device="cuda")[:, None], torch.arange(s0 + m, device="cuda")[None, :]
+        hidden = (key > here) if causal else torch.zeros_like(key > here)
+        if window:
+            hidden = hidden | (key <= here - window)
+        vs = pool.vs[0][pool.table[i].long()[torch.arange(s0 + m, device="cuda") // pool.page]].double()
+        for h in range(n_q):
+            g = h // (n_q // n_kv)
+            x = q[row:row + m, h].double()
+            score = (x @ k[:, g].T / math.sqrt(d)).masked_fill(hidden, -math.inf)
+            p = torch.softmax(score, -1)
+            out[row:row + m, h] = p @ v[:, g]
+            off = x.abs().amax(-1, keepdim=True) * k[:, g].abs().sum(-1).max() / math.sqrt(d) * 2.0 ** -24
+            size = score.masked_fill(hidden, 0.0).abs().amax(-1, keepdim=True)
+            tol[row:row + m, h] = (2 * (off + size * 2.0 ** -21) + 2.0 ** -17 + 2.0 ** -21 + ((s0 + m) / 64 + 5) * 2.0 ** -23) * (p @ vs[:, g, None]) * 127
+        row += m
+    return out, tol
+
+
+@pytest.mark.parametrize("d,most", [(64, 2), (128, 2), (256, 2)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 1), (True, 23), (False, 40)])
+@pytest.mark.parametrize("octaves", [12, 36, 70])
+def test_attention_over_pages_of_very_unlike_values(d, most, causal, window, octaves):
+    """A row whose keys have small values keeps its bits beside pages with large ones, which it does not see or hardly weighs."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=60, n_kv=2, d=d, page=16, n_seq=2, max_pages=30)
+    start, counts = [0, 330], [150, 6]
+    pool.give([150, 336])
+    for i in range(2):
+        for c in range(22):
+            p = int(pool.table[i, c])
+            if p >= 0:
+                pool.vs[:, p] *= 2.0 ** -(octaves * ((c * 5) % 4) / 3.0)
+    q = torch.randn(156, 8, d, device="cuda", generator=pool.g)
+    got, live = _attend(ctx, pool, q, counts, start, causal, window, most=most)
+    _done(ctx)
+    _check(got, live, *_by_what_a_row_sees(pool, q, start, counts, causal, window))
     ctx.close()

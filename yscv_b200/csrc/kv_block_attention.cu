@@ -2,11 +2,13 @@
 //
 // With q = a_q n_q (n_q whole numbers of 24 bits, a row's largest at 8355711), k = s_k n_k and v = s_v n_v as the cache holds them,
 //   scores   q k = a_q s_k sum n_q n_k          n_q = 65536 q2 + 256 q1 + q0, digits in [-128, 127]
-//   output   p v = (s_v / 2^23) sum n_p n_v     n_p = p 2^23 of the softmax weights p <= 1 of a step, bytes p2 p1 p0
+//   output   p v = (2^T / 2^23) sum n_p n_v     n_p = p s_v 2^-T 2^23 of the softmax weights p of a step, bytes p2 p1 p0
 // so both contractions are integer tensor-core products (mma.sync m16n8k32, int32 sums, exact) on the cache's bytes as they lie:
 // nothing is converted or transposed. Against two fp16 terms per operand, which the framework's other int8 cache takes, that is
 // three or two products for two and no conversion of the cache, which there is most of what the kernel issues. What is rounded: the
-// query to 2^-23 of its row's largest, a weight to 2^-24 of its step's largest, and fp32 sums over steps.
+// query to 2^-23 of its row's largest, a weight to 2^-23 of its row's and step's largest weight times scale, and fp32 sums over steps.
+// T is a row's own: with one for a step's largest scale a row that sees, or weighs, only pages whose values are 2^12 times smaller kept 12
+// bits.
 //
 // Work: a step is 64 keys of a (sequence, KV head, block of R (position, head) pairs). All steps of a call are laid end to
 // end, sequence after sequence, and every warp of the GPU takes an equal run of them, so that neither one long conversation nor
@@ -32,7 +34,8 @@ namespace yscv {
 
 constexpr int KA_STEP = 64;                   // keys of a step
 constexpr float KA_Q = 8355711.0f;            // 127 * (65536 + 256 + 1)
-constexpr float KA_P = 8388607.0f;            // 2^23 - 1
+constexpr float KA_P = 8387584.0f;            // 2^23 - 1024: T goes by a logarithm that is good to 2^-15
+constexpr int KA_OCTAVES = 90;                // a step's scales count as powers of two down to 2^-90 of its largest, smaller ones by fewer bits
 constexpr float KA_MAGIC = 12582912.0f;       // 1.5 * 2^23: a sum that starts at its bits is the float MAGIC + sum (|sum| < 2^22)
 constexpr int KA_MAGIC_BITS = 0x4B400000;
 
@@ -77,9 +80,11 @@ KA_MMA(ka_mma_u8, "u8")
 __device__ __forceinline__ void ka_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ float ka_exp2(float x) {
+// e of x = f 2^e, f in [1/2, 1) (zero and subnormal numbers: -126)
+__device__ __forceinline__ int ka_exponent(float x) { return min((__float_as_int(x) >> 23) - 126, 126); }
+__device__ __forceinline__ float ka_log2(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    asm("lg2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
 // two sums that began at MAGIC's bits
@@ -371,40 +376,63 @@ __global__ void __launch_bounds__(KaGeom<D, R>::WARPS * 32, 1) kv_attention_kern
                 }
         }
         // ---- weights, relative to the step's own maximum ----
+        // A value scale is f 2^e: a weight takes both, the sum takes e back. f is in [1/2, 1), or smaller where KA_OCTAVES holds e up
+        float ve[4], vc[4], vl[4], back[4];
         const float vmost = fmaxf(fmaxf(vscale[0], vscale[1]), fmaxf(vscale[2], vscale[3]));
-        float vc[4];
+        const int e_least = max(ka_exponent(fmaxf(vmost, 0.0f)) - KA_OCTAVES, -126);
 #pragma unroll
-        for (int grp = 0; grp < 4; ++grp) vc[grp] = vscale[grp] > 0.0f ? fminf(__fdiv_rn(vscale[grp], vmost), 1.0f) * KA_P : 0.0f;
+        for (int grp = 0; grp < 4; ++grp) {
+            const float vs = fmaxf(vscale[grp], 0.0f);
+            const int e = max(ka_exponent(vs), e_least);
+            back[grp] = __int_as_float((127 - e) << 23);
+            ve[grp] = (float)e;
+            vc[grp] = fminf(vs * back[grp], 1.0f) * KA_P;
+            vl[grp] = fmaxf(ka_log2(vs), ve[grp] - 1.0f);
+        }
         uint32_t pa[4][NR][3];                 // [group][row][digit, the highest first]
         float w0[NR], alpha[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-            float mx = s[r][0];
+            float most[4];
 #pragma unroll
-            for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[r][j]);
+            for (int grp = 0; grp < 4; ++grp) most[grp] = fmaxf(fmaxf(s[r][4 * grp], s[r][4 * grp + 1]), fmaxf(s[r][4 * grp + 2], s[r][4 * grp + 3]));
+            float mx = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const float ref = mx == -INFINITY ? 0.0f : mx, m_new = fmaxf(m[r], mx);
+            // 2^T: the row's largest weight times scale, or up to twice that
+            float T = fmaxf(fmaxf(most[0] - ref + vl[0], most[1] - ref + vl[1]), fmaxf(most[2] - ref + vl[2], most[3] - ref + vl[3]));
+            T = fmaxf(T, __shfl_xor_sync(0xffffffffu, T, 1));
+            T = fmaxf(T, __shfl_xor_sync(0xffffffffu, T, 2));
+            T = fminf(fmaxf(ceilf(T), -126.0f), 126.0f);
+            const float two_T = __int_as_float(((int)T + 127) << 23);
             float sum = 0.0f;
 #pragma unroll
             for (int grp = 0; grp < 4; ++grp) {
+                const uint64_t by_e = f2(ve[grp] - T, ve[grp] - T), by_ref = f2(-ref, -ref);
                 uint32_t x[4];
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    // (the difference of the scores first: it is exact where it counts, whatever their size)
+                    f2_get(f2_add(f2_add(f2(s[r][4 * grp + j], s[r][4 * grp + j + 1]), by_ref), by_e), p[j], p[j + 1]);
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float p = ka_exp2(s[r][4 * grp + j] - ref);
-                    sum += p;
-                    x[j] = __float_as_uint(fmaf(p, vc[grp], 8388608.0f));   // 2^23 + n_p: the low bytes are the digits
+                    p[j] = at_exp2(p[j]);
+                    x[j] = __float_as_uint(fmaf(p[j], vc[grp], 8388608.0f));   // 2^23 + n_p: the low bytes are the digits
                 }
+                sum = fmaf((p[0] + p[1]) + (p[2] + p[3]), two_T * back[grp], sum);
                 const uint32_t y = __byte_perm(x[0], x[1], 0x5140), z = __byte_perm(x[2], x[3], 0x5140);
                 pa[grp][r][2] = __byte_perm(y, z, sel0);
                 pa[grp][r][1] = __byte_perm(y, z, sel1);
                 pa[grp][r][0] = __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), sel0);
             }
-            alpha[r] = m_new == -INFINITY ? 1.0f : ka_exp2(m[r] - m_new);
-            const float beta = m_new == -INFINITY ? 0.0f : ka_exp2(mx - m_new);
+            alpha[r] = m_new == -INFINITY ? 1.0f : at_exp2(m[r] - m_new);
+            const float beta = m_new == -INFINITY ? 0.0f : at_exp2(mx - m_new);
             l[r] = fmaf(l[r], alpha[r], beta * sum);
             m[r] = m_new;
-            w0[r] = beta * (vmost > 0.0f ? vmost : 0.0f) * (1.0f / KA_P);
+            w0[r] = beta * two_T * (1.0f / KA_P);
         }
         // ---- weighted values ----
         alive = __all_sync(0xffffffffu, mbar_wait(v_bar, (uint32_t)i & 1u, a.status));
@@ -533,7 +561,7 @@ __global__ void __launch_bounds__(32 * W * P) kv_attention_merge_kernel(const __
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float old = ka_exp2(m - ref), w = ka_exp2(ml.x - ref);   // (0 for a lane without a record)
+            const float old = at_exp2(m - ref), w = at_exp2(ml.x - ref);   // (0 for a lane without a record)
             m = m_new;
             l = fmaf(l, old, w * ml.y);          // (of the lane's records)
 #pragma unroll
@@ -576,12 +604,12 @@ __global__ void __launch_bounds__(32 * W * P) kv_attention_merge_kernel(const __
         const float ref = all == -INFINITY ? 0.0f : all;
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) sum = fmaf(ka_exp2(red[i][0] - ref), red[i][1], sum);
+        for (int i = 0; i < W; ++i) sum = fmaf(at_exp2(red[i][0] - ref), red[i][1], sum);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         for (int c = tid; c < D; c += 32 * W) {
             float y = 0.0f;
 #pragma unroll
-            for (int i = 0; i < W; ++i) y = fmaf(ka_exp2(red[i][0] - ref), part[i][c], y);
+            for (int i = 0; i < W; ++i) y = fmaf(at_exp2(red[i][0] - ref), part[i][c], y);
             dst[c] = y * inv;
         }
         __syncthreads();
