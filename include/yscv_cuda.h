@@ -751,7 +751,8 @@ int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
  * row without `causal`; with window > 0 only over keys after its own position minus window. scale 0
  * stands for 1 / sqrt(d_head). out rows are out_stride floats apart and may not overlap d_q; a row that sees no
  * key is 0. Cached numbers enter the products as they are, queries and softmax weights to 22 bits or more: as three
- * 8-bit digits and integer products for a few rows a sequence, as two fp16 terms for more. `rows` is the room in d_q and
+ * 8-bit digits and integer products for a few rows a sequence, as two fp16 terms for more; a weight together with its page's value
+ * scale (scales down to 2^-80 of the largest among 128 keys; smaller ones count as that small). `rows` is the room in d_q and
  * d_out, at least d_offsets[n_seq]: a sequence whose offsets lie outside takes no part, status 4. Keys behind the table's
  * end are left out, status 3. Rows with a NaN or an infinity in the query are NaN, and only those. d_head 64, 128 or
  * 256. _workspace says how many bytes of device memory a call needs; calls that may overlap need one each. */

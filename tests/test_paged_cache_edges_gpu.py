@@ -104,7 +104,7 @@ def _by_what_a_row_sees(pool, q, start, counts, causal, window):
     return out, tol
 
 
-@pytest.mark.parametrize("d,most", [(64, 2), (128, 2), (256, 2)])
+@pytest.mark.parametrize("d,most", [(64, 2), (128, 2), (256, 2), (64, 80), (128, 80)])
 @pytest.mark.parametrize("causal,window", [(True, 0), (True, 1), (True, 23), (False, 40)])
 @pytest.mark.parametrize("octaves", [12, 36, 70])
 def test_attention_over_pages_of_very_unlike_values(d, most, causal, window, octaves):

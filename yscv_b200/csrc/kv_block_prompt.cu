@@ -12,7 +12,8 @@
 //   warps 2, 3   keys and values of the tiles as they are cached, by bulk copies a tile ahead, and what the others have to know
 //   warps 4-7    the tile's bytes as fp16 operands
 //   warps 8-15   softmax, a thread a row, two tiles at a time: the queries' two terms to TMEM for a segment's first tile; scores from
-//                TMEM, the tile's own maximum and sum, weights back to where the scores were. They keep nothing from tile to tile
+//                TMEM, the tile's own maximum (of weight times value scale) and sum, weights back to where the scores were. They keep
+//                nothing from tile to tile
 //   warps 16-19  the output in registers, a thread per row: o = o + O 2^(m - M), M at most 2^8 below the running maximum, and results
 // With the output in the softmax threads' registers those have too few left to keep several exponentials in flight: 2048 x 2048
 // keys, 64 / 8 heads of 128, 507 us, a tile of 128 rows 6300 cycles. With all eight softmax warps on one tile, which then hand its
@@ -482,8 +483,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
 #pragma unroll
                     for (int d = 4; d > 0; d >>= 1) vmost = fmaxf(vmost, __shfl_xor_sync(0xffffffffu, vmost, d));
                     if (lane < 8) {
-                        // (at least 2^-60: a group whose values are 0 counts in the sum all the same)
-                        const float ratio = fmaxf(__fdiv_rn(vs, fmaxf(vmost, 7.5e-37f)), 8.6736174e-19f);
+                        // (at least 2^-80: a group whose values are 0 counts in the sum all the same, and the inverse stays far below
+                        // what sums over a sequence can hold)
+                        const float ratio = fmaxf(__fdiv_rn(vs, fmaxf(vmost, 7.5e-37f)), 8.2718061e-25f);
                         o.ks[lane] = ks;
                         o.lv[lane] = there ? log2f(ratio) : -INFINITY;
                         o.iv[lane] = there ? __fdiv_rn(1.0f, ratio) : 0.0f;
@@ -643,26 +645,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
             // (never 0, where pages have no scale or products leave fp32's range: a hidden key's -inf has to stay one. What a seen key's
             // score, at most 2^29 here, becomes by it is 2^-97 at most, a weight's exponent of nothing)
             auto times = [&](float k) { return fmaxf(to_log2 * k, FLT_MIN); };
+            // The largest weight times value scale, not the largest weight: what a row sees has its 22 bits whatever lies beside it
             float mx = -INFINITY, v[16], u[16];
             kp_ld16(s_at, v);
 #pragma unroll 1
             for (int g = 0; g < groups; g += 2) {
-                const float2 k2 = *reinterpret_cast<const float2 *>(ks + g);
-                auto most = [&](const float (&z)[16], float k) {
+                const float2 k2 = *reinterpret_cast<const float2 *>(ks + g), l2 = *reinterpret_cast<const float2 *>(lv + g);
+                auto most = [&](const float (&z)[16], float k, float lv) {
                     float x = fmaxf(z[0], z[1]), y = fmaxf(z[2], z[3]);
 #pragma unroll
                     for (int e = 4; e < 16; e += 4) {
                         x = fmaxf(x, fmaxf(z[e], z[e + 1]));
                         y = fmaxf(y, fmaxf(z[e + 2], z[e + 3]));
                     }
-                    mx = fmaxf(mx, fmaxf(x, y) * times(k));
+                    mx = fmaxf(mx, fmaf(fmaxf(x, y), times(k), lv));
                 };
                 kp_wait_ld16(v);
                 kp_ld16(s_at + 16 * g + 16, u);
-                most(v, k2.x);
+                most(v, k2.x, l2.x);
                 kp_wait_ld16(u);
                 kp_ld16(s_at + (g + 2 < groups ? 16 * g + 32 : 0), v);     // (at the end the first ones again)
-                most(u, k2.y);
+                most(u, k2.y, l2.y);
             }
             const float off = mx == -INFINITY ? 0.0f : 10.0f - mx;
             float sum = 0.0f;
