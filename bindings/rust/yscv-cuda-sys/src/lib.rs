@@ -238,7 +238,9 @@ extern "C" {
     pub fn yscv_cuda_decoder_layers_dev(ctx: *mut yscv_cuda_ctx, layers: *const yscv_cuda_decode_layer, n_layers: usize, hidden: usize, inter: usize, n_q: usize, n_kv: usize, d_head: usize, max_seq: usize, eps: f32, rope_theta: f32, kv_int8: c_int, batch: usize, seq: usize, d_pos: *const i32, d_x: *mut f32, d_final_gamma: *const f32, d_last: *mut f32, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn yscv_cuda_rope_dev(ctx: *mut yscv_cuda_ctx, d_x: *const f32, x_stride: usize, rows: usize, n_heads: usize, d_head: usize, d_pos: *const i32, rope: *const yscv_cuda_rope, d_out: *mut f32, out_stride: usize) -> c_int;
     pub fn yscv_cuda_kv_block_append_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_k: *const f32, d_v: *const f32, row_stride: usize, d_offsets: *const i32, d_start: *const i32, most_rows: usize) -> c_int;
+    pub fn yscv_cuda_kv_block_append_rows_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_k: *const f32, d_v: *const f32, row_stride: usize, d_offsets: *const i32, d_start: *const i32, rows: usize, most_rows: usize) -> c_int;
     pub fn yscv_cuda_kv_block_read_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_offsets: *const i32, d_start: *const i32, most_rows: usize, d_k_out: *mut f32, d_v_out: *mut f32, row_stride: usize) -> c_int;
+    pub fn yscv_cuda_kv_block_read_rows_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_offsets: *const i32, d_start: *const i32, rows: usize, most_rows: usize, d_k_out: *mut f32, d_v_out: *mut f32, row_stride: usize) -> c_int;
     pub fn yscv_cuda_kv_block_attention_workspace(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, n_q: usize, rows: usize, most_rows: usize, bytes: *mut usize) -> c_int;
     pub fn yscv_cuda_kv_block_attention_dev(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, layer: usize, d_q: *const f32, q_stride: usize, n_q: usize, d_offsets: *const i32, d_start: *const i32, rows: usize, most_rows: usize, causal: c_int, window: usize, scale: f32, d_out: *mut f32, out_stride: usize, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn yscv_cuda_kv_pages_workspace(ctx: *mut yscv_cuda_ctx, pool: *const yscv_cuda_kv_pool, bytes: *mut usize) -> c_int;

@@ -736,15 +736,22 @@ typedef struct yscv_cuda_kv_pool {
  * A page that already holds tokens in front of the new ones keeps its scale, or takes the larger one of
  * the new tokens and rounds what it holds once more. A NaN is held as 0, an infinity as +-127; neither
  * counts for the scale. Pages that sequences share have to be made their own first
- * (yscv_cuda_kv_pages_extend_dev does). d_head is a multiple of 16, at most 256. */
+ * (yscv_cuda_kv_pages_extend_dev does). d_head is a multiple of 16, at most 256. A sequence whose offsets fall, or lie outside the
+ * operands' rows, takes no part, status 4: _append_rows is told how many there are, without them d_offsets[n_seq] is believed. */
 int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_k,
                                   const float *d_v, size_t row_stride, const int32_t *d_offsets,
                                   const int32_t *d_start, size_t most_rows);
+int yscv_cuda_kv_block_append_rows_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer,
+                                       const float *d_k, const float *d_v, size_t row_stride, const int32_t *d_offsets,
+                                       const int32_t *d_start, size_t rows, size_t most_rows);
 /* The cached rows at the positions of a ragged call as f32, number times scale: the inverse. A row
- * that has no page is left as it was. */
+ * that has no page is left as it was. Offsets as above. */
 int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer,
                                 const int32_t *d_offsets, const int32_t *d_start, size_t most_rows, float *d_k_out,
                                 float *d_v_out, size_t row_stride);
+int yscv_cuda_kv_block_read_rows_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer,
+                                     const int32_t *d_offsets, const int32_t *d_start, size_t rows, size_t most_rows,
+                                     float *d_k_out, float *d_v_out, size_t row_stride);
 
 /* Attention of the new rows over the pages of one layer: row s of sequence i (q_stride floats apart, n_q
  * heads of d_head, n_q a multiple of n_kv) over the keys 0 .. d_start[i] + s, or all up to the sequence's last new

@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from paged_pool import Pool, attention
-from test_paged_cache_gpu import _append, _attend, _check, _context, _done
+from paged_pool import Pool, attention, i32
+from test_paged_cache_gpu import _append, _attend, _check, _context, _done, _expect_append, _refused, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -122,4 +122,62 @@ def test_attention_over_pages_of_very_unlike_values(d, most, causal, window, oct
     got, live = _attend(ctx, pool, q, counts, start, causal, window, most=most)
     _done(ctx)
     _check(got, live, *_by_what_a_row_sees(pool, q, start, counts, causal, window))
+    ctx.close()
+
+
+# offsets of three sequences, and whether the operands' six rows have to be told
+WRONG_OFFSETS = [
+    ([0, 2, 4, 7], True), ([0, 2, 4, 0x7FFFFFFF], True), ([9, 9, 9, 9], True), ([-4, 2, 4, 6], False), ([0, 2, 9, 6], False), ([0, 2, 1, 6], False),
+    ([0x7FFFFFFF, -(1 << 31), 4, 6], False), ([0, 2, 4, -1], False),
+]
+
+
+@pytest.mark.parametrize("off,told", WRONG_OFFSETS)
+@pytest.mark.parametrize("most", [0, 2, 300])
+def test_append_and_read_leave_sequences_out_whose_offsets_are_wrong(off, told, most):
+    """Falling offsets and ones outside the rows: status 4, the pages and the rows of the others as they should be, nothing else touched."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=40, n_kv=2, d=64, page=16, n_seq=3, max_pages=12)
+    start = [97, 47, 147]
+    pool.give([110, 60, 160])
+    x = torch.randn(2, 6 + 4, 128, device="cuda", generator=pool.g)
+    x[:, 6:] = 1e6                                      # rows that would make every scale grow
+    handle, o, st = pool.handle(), i32(off), i32(start)
+    for rows in (6,) if told else (6, None):
+        room = off[3] if rows is None else rows
+        served = [i for i in range(3) if 0 <= off[i] <= off[i + 1] <= room]
+        counts = [off[i + 1] - off[i] if i in served else 0 for i in range(3)]
+        before = pool.state()
+        torch.cuda.synchronize()
+        ctx.kv_block_append_dev(handle, 0, x[0].data_ptr(), x[1].data_ptr(), 128, o.data_ptr(), st.data_ptr(), most, rows=rows)
+        _done(ctx, 4)
+        k, v = (torch.cat([t[off[i]:off[i] + counts[i]] for i in served] + [t[:0]]).view(-1, 2, 64) for t in x)
+        _same(pool, _expect_append(before, pool, k, v, counts, start))
+        out = torch.full((2, 6 + 4, 128), 5.0, device="cuda")
+        want = out.clone()
+        torch.cuda.synchronize()
+        ctx.kv_block_read_dev(handle, 0, o.data_ptr(), st.data_ptr(), most, out[0].data_ptr(), out[1].data_ptr(), 128, rows=rows)
+        _done(ctx, 4)
+        for i in served:
+            for w, c in zip(want, pool.rows(i, start[i] + counts[i])):
+                w[off[i]:off[i] + counts[i]] = c[start[i]:].float().reshape(-1, 128)
+        # (a row that two sequences claim, as [0, 2, 1, 6] has it, holds what one of them has there)
+        once = [sum(off[i] <= r < off[i] + counts[i] for i in served) < 2 for r in range(10)]
+        assert torch.equal(out[:, once], want[:, once])
+        pool.restore(before)
+    ctx.close()
+
+
+def test_append_and_read_refuse_rows_beyond_counting():
+    ctx = _context()
+    pool = Pool(ctx)
+    handle, x, n = pool.handle(), torch.zeros(4096, device="cuda"), i32([0] * 8)
+    p, i = x.data_ptr(), n.data_ptr()
+    torch.cuda.synchronize()
+    for rows in (1 << 31, (1 << 64) - 1):
+        _refused(lambda: ctx.kv_block_append_dev(handle, 0, p, p, 128, i, i, 1, rows=rows), -3)
+        _refused(lambda: ctx.kv_block_read_dev(handle, 0, i, i, 1, p, p, 128, rows=rows), -3)
+    ctx.kv_block_append_dev(handle, 0, p, p, 128, i, i, 1, rows=0)
+    ctx.kv_block_read_dev(handle, 0, i, i, 1, p, p, 128, rows=0)
+    _done(ctx)
     ctx.close()

@@ -21,6 +21,7 @@ namespace yscv {
 struct KvRows {
     const int32_t *offsets, *start;
     size_t stride;                 // floats between rows
+    int room;                      // rows of the operands, -1: as many as the last offset says
 };
 
 // The whole number next to the border b on the side that the sign of `off` says, the even one on the border itself
@@ -104,15 +105,22 @@ __device__ __forceinline__ uint32_t kv_requantise(uint32_t w, int count, float r
 // Pages of the rows of sequence `seq`: the first and how many
 struct KvSpan {
     int row0, rows, p0;            // first row, rows, position of the first
-    bool live;
+    bool live, inside;             // takes part; has rows of the operands
 };
-__device__ __forceinline__ KvSpan kv_span(const KvRows &r, int seq) {
+__device__ __forceinline__ KvSpan kv_span(const KvRows &r, int seq, int n_seq) {
     KvSpan s;
+    const int end = r.offsets[seq + 1], last = r.offsets[n_seq];
     s.row0 = r.offsets[seq];
-    s.rows = r.offsets[seq + 1] - s.row0;
     s.p0 = r.start[seq];
-    s.live = s.rows > 0 && s.p0 >= 0;
+    // (as kv_rows() of kv_attention.cuh: offsets that fall, or lie outside the operands, are nobody's rows)
+    s.inside = s.row0 >= 0 && s.row0 <= end && end <= (r.room >= 0 ? r.room : last);
+    s.rows = end - s.row0;
+    s.live = s.inside && s.rows > 0 && s.p0 >= 0;
     return s;
+}
+// What is said of a sequence that takes no part, once
+__device__ __forceinline__ void kv_span_status(const KvSpan &s, int per_seq, int *status) {
+    if (!s.inside && threadIdx.x == 0 && blockIdx.x % per_seq == 0 && blockIdx.y == 0 && blockIdx.z == 0) atomicExch(status, YSCV_DEV_BAD_NUMBER);
 }
 
 constexpr int KVB_KEEP = 8;        // float4 a thread keeps in registers between the maximum and the quantising
@@ -138,8 +146,11 @@ __global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l,
     pdl_trigger();
     const int tid = threadIdx.x, seq = blockIdx.x / per_seq, head = blockIdx.y;
     const bool values = blockIdx.z != 0;
-    const KvSpan sp = kv_span(rows, seq);
-    if (!sp.live) return;
+    const KvSpan sp = kv_span(rows, seq, l.n_seq);
+    if (!sp.live) {
+        kv_span_status(sp, per_seq, status);
+        return;
+    }
     const long long end = (long long)sp.p0 + sp.rows;
     // a thread has four d of every `step`-th token
     const int d = D ? D : l.d, d4 = d >> 2, step = T / d4, c = tid % d4, first = tid / d4 < step ? tid / d4 : 1 << 30, pitch = kv_stage_pitch(d);
@@ -269,8 +280,11 @@ __global__ void __launch_bounds__(128, 8) kv_read_kernel(const KvLayer l, const 
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, seq = blockIdx.x / per_seq, head = blockIdx.y;
     const bool values = blockIdx.z != 0;
-    const KvSpan sp = kv_span(rows, seq);
-    if (!sp.live) return;
+    const KvSpan sp = kv_span(rows, seq, l.n_seq);
+    if (!sp.live) {
+        kv_span_status(sp, per_seq, status);
+        return;
+    }
     const long long end = (long long)sp.p0 + sp.rows;
     float *dst = (values ? v_out : k_out) + (size_t)sp.row0 * rows.stride + (size_t)head * l.d;
     for (long long pg = (sp.p0 >> l.page_shift) + blockIdx.x % per_seq; (pg << l.page_shift) < end; pg += per_seq) {
@@ -336,8 +350,10 @@ static int pages_per_seq(const KvLayer &l, size_t most_rows) {
     const size_t n = (most_rows + l.page - 2) / l.page + 1;
     return (int)(n < (size_t)l.max_pages ? n : (size_t)l.max_pages);
 }
+constexpr size_t KVB_ROWS_UNKNOWN = ~(size_t)0;
+static int room_of(size_t rows) { return rows == KVB_ROWS_UNKNOWN ? -1 : (int)rows; }
 static int check_rows(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const int32_t *d_offsets, const int32_t *d_start, size_t stride,
-                      size_t most_rows, KvLayer *l) {
+                      size_t rows, size_t most_rows, KvLayer *l) {
     if (!ctx) return fail(YSCV_CUDA_ERR_BAD_ARG, "ctx is null");
     if (const int rc = kv_check_pool(pool)) return rc;
     if (const int rc = kv_layer_of(pool, layer, l)) return rc;
@@ -345,20 +361,15 @@ static int check_rows(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t 
     if (!kv_aligned({d_offsets, d_start})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     if (stride < pool->n_kv * pool->d_head) return fail(YSCV_CUDA_ERR_BAD_ARG, "row stride %zu is shorter than n_kv * d_head", stride);
     if (most_rows >= (1u << 31)) return fail(YSCV_CUDA_ERR_BAD_ARG, "most_rows is too large");
+    if (rows != KVB_ROWS_UNKNOWN && rows >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows");
     if (pool->n_seq * (size_t)pages_per_seq(*l, most_rows ? most_rows : 1) >= (1u << 31)) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many pages for one call");
     return YSCV_CUDA_OK;
 }
 
-}  // namespace yscv
-
-using namespace yscv;
-
-extern "C" {
-
-int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_k, const float *d_v,
-                                  size_t row_stride, const int32_t *d_offsets, const int32_t *d_start, size_t most_rows) {
+static int kv_append(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_k, const float *d_v, size_t row_stride,
+                     const int32_t *d_offsets, const int32_t *d_start, size_t n_rows, size_t most_rows) {
     KvLayer l;
-    if (const int rc = check_rows(ctx, pool, layer, d_offsets, d_start, row_stride, most_rows, &l)) return rc;
+    if (const int rc = check_rows(ctx, pool, layer, d_offsets, d_start, row_stride, n_rows, most_rows, &l)) return rc;
     if (!d_k || !d_v) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
     if (!kv_aligned({d_k, d_v})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
@@ -368,7 +379,7 @@ int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
     const size_t most = (most_rows < pool->page ? most_rows : pool->page) * pool->d_head;
     const int threads = most <= 2 * 64 * 4 ? 64 : most <= 128 * 4 * KVB_KEEP ? 128 : most <= 256 * 4 * KVB_KEEP ? 256 : 512;
     const dim3 grid((unsigned)(l.n_seq * per), (unsigned)l.n_kv, 2);
-    const KvRows rows = {d_offsets, d_start, row_stride};
+    const KvRows rows = {d_offsets, d_start, row_stride, room_of(n_rows)};
     // (room for a whole page: a sequence may have more rows than were expected)
     const size_t smem = (size_t)l.page * kv_stage_pitch(l.d);
     auto of = [&](auto size) {
@@ -386,15 +397,15 @@ int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
     return YSCV_CUDA_OK;
 }
 
-int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const int32_t *d_offsets,
-                                const int32_t *d_start, size_t most_rows, float *d_k_out, float *d_v_out, size_t row_stride) {
+static int kv_read(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const int32_t *d_offsets, const int32_t *d_start, size_t n_rows,
+                   size_t most_rows, float *d_k_out, float *d_v_out, size_t row_stride) {
     KvLayer l;
-    if (const int rc = check_rows(ctx, pool, layer, d_offsets, d_start, row_stride, most_rows, &l)) return rc;
+    if (const int rc = check_rows(ctx, pool, layer, d_offsets, d_start, row_stride, n_rows, most_rows, &l)) return rc;
     if (!d_k_out || !d_v_out) return fail(YSCV_CUDA_ERR_BAD_ARG, "null operand");
     if (!kv_aligned({d_k_out, d_v_out})) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "operands must be 4-byte aligned");
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const int per = pages_per_seq(l, most_rows);
-    const KvRows rows = {d_offsets, d_start, row_stride};
+    const KvRows rows = {d_offsets, d_start, row_stride, room_of(n_rows)};
     YSCV_CUDA_TRY(launch_pdl(kv_read_kernel, dim3((unsigned)(l.n_seq * per), (unsigned)l.n_kv, 2), dim3(128), 0, ctx->stream, l, rows, per, d_k_out,
                              d_v_out, (int)(((reinterpret_cast<uintptr_t>(d_k_out) | reinterpret_cast<uintptr_t>(d_v_out)) & 15) == 0 && row_stride % 4 == 0),
                              ctx->d_status));
@@ -402,6 +413,32 @@ int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *poo
     ctx->launches++;
     ctx->last_kernel = "kv_block_read";
     return YSCV_CUDA_OK;
+}
+
+}  // namespace yscv
+
+using namespace yscv;
+
+extern "C" {
+
+int yscv_cuda_kv_block_append_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_k, const float *d_v,
+                                  size_t row_stride, const int32_t *d_offsets, const int32_t *d_start, size_t most_rows) {
+    return kv_append(ctx, pool, layer, d_k, d_v, row_stride, d_offsets, d_start, KVB_ROWS_UNKNOWN, most_rows);
+}
+int yscv_cuda_kv_block_append_rows_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_k, const float *d_v,
+                                       size_t row_stride, const int32_t *d_offsets, const int32_t *d_start, size_t rows, size_t most_rows) {
+    if (rows == KVB_ROWS_UNKNOWN) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows");
+    return kv_append(ctx, pool, layer, d_k, d_v, row_stride, d_offsets, d_start, rows, most_rows);
+}
+
+int yscv_cuda_kv_block_read_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const int32_t *d_offsets,
+                                const int32_t *d_start, size_t most_rows, float *d_k_out, float *d_v_out, size_t row_stride) {
+    return kv_read(ctx, pool, layer, d_offsets, d_start, KVB_ROWS_UNKNOWN, most_rows, d_k_out, d_v_out, row_stride);
+}
+int yscv_cuda_kv_block_read_rows_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const int32_t *d_offsets,
+                                     const int32_t *d_start, size_t rows, size_t most_rows, float *d_k_out, float *d_v_out, size_t row_stride) {
+    if (rows == KVB_ROWS_UNKNOWN) return fail(YSCV_CUDA_ERR_UNSUPPORTED, "too many rows");
+    return kv_read(ctx, pool, layer, d_offsets, d_start, rows, most_rows, d_k_out, d_v_out, row_stride);
 }
 
 }  // extern "C"

@@ -138,7 +138,9 @@ SIGNATURES = {
                                                  C.c_int, _vp]),
     "yscv_cuda_rope_dev": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _sz]),
     "yscv_cuda_kv_block_append_dev": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
+    "yscv_cuda_kv_block_append_rows_dev": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz, _sz]),
     "yscv_cuda_kv_block_read_dev": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _sz]),
+    "yscv_cuda_kv_block_read_rows_dev": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _vp, _sz]),
     "yscv_cuda_kv_block_attention_workspace": (C.c_int, [_vp, _vp, _sz, _sz, _sz, C.POINTER(_sz)]),
     "yscv_cuda_kv_block_attention_dev": (C.c_int, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _sz, C.c_int, _sz, C.c_float,
                                                    _vp, _sz, _vp, _sz]),
@@ -840,15 +842,25 @@ class Context:
         """Rotary positions of the first n_heads heads of every row; d_pos [rows], negative: a row that is left alone."""
         _check(self.lib.yscv_cuda_rope_dev(self.handle, d_x, x_stride, rows, n_heads, d_head, d_pos, C.byref(rope), d_out, out_stride))
 
-    def kv_block_append_dev(self, pool: KvPool, layer, d_k, d_v, row_stride, d_offsets, d_start, most_rows):
-        """Keys and values of ragged rows into their pages (int8, one scale per page and KV head)."""
-        _check(self.lib.yscv_cuda_kv_block_append_dev(self.handle, C.byref(pool), layer, d_k, d_v, row_stride, d_offsets, d_start,
-                                                      most_rows))
+    def kv_block_append_dev(self, pool: KvPool, layer, d_k, d_v, row_stride, d_offsets, d_start, most_rows, rows=None):
+        """Keys and values of ragged rows into their pages (int8, one scale per page and KV head). `rows`: how many d_k and d_v
+        hold; without it the last offset is believed."""
+        if rows is None:
+            _check(self.lib.yscv_cuda_kv_block_append_dev(self.handle, C.byref(pool), layer, d_k, d_v, row_stride, d_offsets, d_start,
+                                                          most_rows))
+        else:
+            _check(self.lib.yscv_cuda_kv_block_append_rows_dev(self.handle, C.byref(pool), layer, d_k, d_v, row_stride, d_offsets, d_start,
+                                                               rows, most_rows))
 
-    def kv_block_read_dev(self, pool: KvPool, layer, d_offsets, d_start, most_rows, d_k_out, d_v_out, row_stride):
-        """The cached rows at the positions of a ragged call, as f32."""
-        _check(self.lib.yscv_cuda_kv_block_read_dev(self.handle, C.byref(pool), layer, d_offsets, d_start, most_rows, d_k_out, d_v_out,
-                                                    row_stride))
+    def kv_block_read_dev(self, pool: KvPool, layer, d_offsets, d_start, most_rows, d_k_out, d_v_out, row_stride, rows=None):
+        """The cached rows at the positions of a ragged call, as f32. `rows`: how many d_k_out and d_v_out hold; without it the last
+        offset is believed."""
+        if rows is None:
+            _check(self.lib.yscv_cuda_kv_block_read_dev(self.handle, C.byref(pool), layer, d_offsets, d_start, most_rows, d_k_out, d_v_out,
+                                                        row_stride))
+        else:
+            _check(self.lib.yscv_cuda_kv_block_read_rows_dev(self.handle, C.byref(pool), layer, d_offsets, d_start, rows, most_rows, d_k_out,
+                                                             d_v_out, row_stride))
 
     def kv_block_attention_workspace(self, pool: KvPool, n_q, rows, most_rows) -> int:
         """Bytes of device memory a kv_block_attention_dev call needs."""
