@@ -776,9 +776,10 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
  *   pages in the order of the sequences. A last page that is not full and that others share is
  *   copied to a page of its own first (by every one of them that grows: the page itself is freed when
  *   none is left). d_length grows; d_start receives the old length and d_pos [rows] the position of every
- *   row, as the calls above take them. A sequence with no rows, one whose table is too short (status 3), and from
- *   the first sequence that finds no page on all that need one (status 5) stay as they are, with -1 in
- *   d_start and d_pos; so do rows behind the last one.
+ *   row, as the calls above take them (rows 0: no positions are asked for). A sequence with no rows, one whose
+ *   offsets fall or lie outside the call's rows (status 4), one whose table is too short (status 3), and from the
+ *   first sequence that finds no page on all that need one (status 5) stay as they are, with -1 in d_start and
+ *   d_pos; so do rows behind the last one.
  * trim: sequence d_seqs[j] keeps its first d_keep[j] tokens (d_keep null: none); pages that nobody holds
  *   any more are free.
  * fork: the empty sequence d_dst[j] shares all pages of d_src[j]. A source that is a destination of the same

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from paged_pool import Pool, attention, i32
-from test_paged_cache_gpu import _append, _attend, _check, _context, _done, _expect_append, _refused, _same
+from test_paged_cache_gpu import Book, _append, _attend, _check, _context, _done, _expect_append, _refused, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -180,4 +180,45 @@ def test_append_and_read_refuse_rows_beyond_counting():
     ctx.kv_block_append_dev(handle, 0, p, p, 128, i, i, 1, rows=0)
     ctx.kv_block_read_dev(handle, 0, i, i, 1, p, p, 128, rows=0)
     _done(ctx)
+    ctx.close()
+
+
+@pytest.mark.parametrize("off", [off for off, _ in WRONG_OFFSETS] + [[0, 2, 100, 4], [0, 2, 4, 3]])
+def test_pages_grow_for_sequences_whose_offsets_are_right(off):
+    """Falling offsets and ones outside the rows: status 4, -1 and no pages for those, the others' pages and positions as they should be."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=20, n_kv=1, d=16, page=16, n_seq=4, max_pages=8)
+    pool.give([31, 16, 0, 40])
+    off = off + [6]
+    book = Book(pool)
+    inside = [0 <= a <= b <= 6 for a, b in zip(off, off[1:])]
+    new = [off[i + 1] - off[i] if inside[i] else 0 for i in range(4)]
+    before = pool.state()
+    start, pos = torch.full((4,), 77, dtype=torch.int32, device="cuda"), torch.full((6,), 77, dtype=torch.int32, device="cuda")
+    handle, o = pool.handle(), i32(off)
+    ws = torch.empty(ctx.kv_pages_workspace(handle), dtype=torch.uint8, device="cuda").random_(0, 256)
+    torch.cuda.synchronize()
+    ctx.kv_pages_extend_dev(handle, o.data_ptr(), 6, start.data_ptr(), pos.data_ptr(), ws.data_ptr(), ws.numel())
+    _done(ctx, 0 if all(inside) else 4)
+    want, status = book.extend(new)
+    assert status == 0 and start.tolist() == want
+    book.same(pool, before)
+    for r in range(6):
+        here = [i for i in range(4) if want[i] >= 0 and off[i] <= r < off[i + 1]]
+        assert pos[r] == (want[here[0]] + r - off[here[0]] if here else -1)
+    ctx.close()
+
+
+def test_pages_grow_without_positions():
+    ctx = _context()
+    pool = Pool(ctx, n_pages=20, n_kv=1, d=16, page=16, n_seq=3, max_pages=8)
+    pool.give([31, 16, 0])
+    book, before = Book(pool), pool.state()
+    handle, o, start = pool.handle(), i32([0, 2, 40, 41]), i32([77] * 3)
+    ws = torch.empty(ctx.kv_pages_workspace(handle), dtype=torch.uint8, device="cuda").random_(0, 256)
+    torch.cuda.synchronize()
+    ctx.kv_pages_extend_dev(handle, o.data_ptr(), 0, start.data_ptr(), None, ws.data_ptr(), ws.numel())
+    _done(ctx)
+    assert book.extend([2, 38, 1]) == (start.tolist(), 0)
+    book.same(pool, before)
     ctx.close()

@@ -54,8 +54,8 @@ struct KvPages {
     int n_pages, n_seq, max_pages, page_shift;
 };
 
-// Workspace: how many copies, pages in use, pieces that copying blocks have taken; the copies' sources and destinations, the free pages that are given out, where a
-// page went, the shared last page of a sequence
+// Workspace: how many copies, pages in use, pieces that copying blocks have taken, whether offsets are wrong; the copies' sources and
+// destinations, the free pages that are given out, where a page went, the shared last page of a sequence
 struct KvWork {
     int32_t *copies, *src, *dst, *free, *moved, *last;
 };
@@ -150,12 +150,14 @@ __device__ __forceinline__ int used_below(const KvUsed &u, int lo, int hi, int t
 // Growth of a sequence but for its last page: tokens it has and gets, pages it has and will have
 struct KvGrowth {
     int length, rows, held, wanted;
-    bool fits;
+    bool fits, inside;             // the table has room; the offsets neither fall nor lie outside the call's rows
 };
-__device__ __forceinline__ KvGrowth growth_of(const KvPages &a, const int32_t *offsets, int i) {
+__device__ __forceinline__ KvGrowth growth_of(const KvPages &a, const int32_t *offsets, int rows, int i) {
     KvGrowth g;
     g.length = a.length[i];
-    g.rows = max(0, offsets[i + 1] - offsets[i]);
+    const int row0 = offsets[i], row1 = offsets[i + 1];
+    g.inside = row0 >= 0 && row0 <= row1 && row1 <= rows;
+    g.rows = g.inside ? row1 - row0 : 0;
     const int page = 1 << a.page_shift;
     const long long end = (long long)g.length + g.rows;
     g.fits = g.length >= 0 && end <= ((long long)a.max_pages << a.page_shift);
@@ -166,8 +168,8 @@ __device__ __forceinline__ KvGrowth growth_of(const KvPages &a, const int32_t *o
 
 constexpr int KVP_LISTED = 2048;   // free pages that are given out from shared memory
 
-__global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a, const int32_t *__restrict__ offsets, int32_t *__restrict__ start,
-                                                                const KvWork w, int *__restrict__ status) {
+__global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a, const int32_t *__restrict__ offsets, int rows,
+                                                                int32_t *__restrict__ start, const KvWork w, int *__restrict__ status) {
     __shared__ uint32_t sums[KVP_WARPS];
     __shared__ uint32_t seen[KVP_SEEN / 32];
     __shared__ int listed[KVP_LISTED];
@@ -176,18 +178,20 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a,
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31;
     if (tid == 0) copies = 0;
+    if (rows == 0) rows = offsets[a.n_seq];       // (no positions are asked for: the last offset is believed)
     // what the sequences need, in their order: a thread takes a run of them (its first one's growth and shared last page stay with it)
     const int per = (a.n_seq + KVP_THREADS - 1) / KVP_THREADS, i0 = min(tid * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
     long long need = 0, wanted;
     KvGrowth first = {};
     int first_last = -1;
-    if (i0 < i1) first = growth_of(a, offsets, i0);
+    bool wrong = false;
+    if (i0 < i1) first = growth_of(a, offsets, rows, i0);
     const KvUsed u = {a.refs, seen, a.n_pages};
     int lo, hi;
     word_run(a.n_pages, lo, hi);
     const int used = look_at_pages(u, lo, hi);
     for (int i = i0; i < i1; ++i) {
-        const KvGrowth g = i == i0 ? first : growth_of(a, offsets, i);
+        const KvGrowth g = i == i0 ? first : growth_of(a, offsets, rows, i);
         int last = -1;
         if (g.rows > 0 && g.fits && (g.length & ((1 << a.page_shift) - 1))) {
             const int p = a.table[(size_t)i * a.max_pages + g.held - 1];
@@ -197,6 +201,10 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a,
         else w.last[i] = last;
         if (g.rows > 0 && g.fits) need += g.wanted - g.held + (last >= 0);
         if (g.rows > 0 && !g.fits) atomicExch(status, YSCV_DEV_POS_OVERFLOW);
+        if (!g.inside) {
+            wrong = true;
+            atomicExch(status, YSCV_DEV_BAD_NUMBER);
+        }
     }
     const long long before = block_prefix(need, sums, wanted);
     // the free pages, as many as are wanted, in their order
@@ -212,7 +220,7 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a,
     auto free_page = [&](long long at) { return at < KVP_LISTED ? listed[at] : w.free[at]; };
     long long upto = before;
     for (int i = i0; i < i1; ++i) {
-        const KvGrowth g = i == i0 ? first : growth_of(a, offsets, i);
+        const KvGrowth g = i == i0 ? first : growth_of(a, offsets, rows, i);
         const int last = i == i0 ? first_last : w.last[i];
         long long at = upto;
         const int mine = g.rows > 0 && g.fits ? g.wanted - g.held + (last >= 0) : 0;
@@ -236,8 +244,8 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a,
         }
         a.length[i] = g.length + g.rows;
     }
-    __syncthreads();
-    if (tid == 0) { w.copies[0] = copies; w.copies[2] = 0; }
+    wrong = __syncthreads_or(wrong);
+    if (tid == 0) { w.copies[0] = copies; w.copies[2] = 0; w.copies[3] = wrong; }
 }
 
 // ---- compact --------------------------------------------------------------------------------------
@@ -383,7 +391,14 @@ __global__ void __launch_bounds__(256) kv_apply_kernel(const KvApply a, int *__r
     const long long thread = (long long)blockIdx.x * 256 + tid, threads = (long long)gridDim.x * 256;
     if (a.pos) {
         const int last = a.offsets[a.n_seq];
+        const bool wrong = a.copies[3] != 0;
         for (long long r = thread; r < a.rows; r += threads) {
+            if (wrong) {                   // offsets in no order: the first sequence that has the row and takes part
+                int i = 0;
+                while (i < a.n_seq && (a.start[i] < 0 || r < a.offsets[i] || r >= a.offsets[i + 1])) ++i;
+                a.pos[r] = i < a.n_seq ? a.start[i] + (int)(r - a.offsets[i]) : -1;
+                continue;
+            }
             int lo = 0, hi = a.n_seq;      // the last sequence whose rows begin at r or before
             while (hi - lo > 1) {
                 const int m = (lo + hi) >> 1;
@@ -486,7 +501,8 @@ int yscv_cuda_kv_pages_extend_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *p
     if (const int rc = check_work(pool, d_workspace, workspace_bytes)) return rc;
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
     const KvWork w = kv_work_of(pool, d_workspace);
-    YSCV_CUDA_TRY(launch_pdl(kv_extend_kernel, dim3(1), dim3(KVP_THREADS), 0, ctx->stream, pages_of(pool), d_offsets, d_start, w, ctx->d_status));
+    YSCV_CUDA_TRY(launch_pdl(kv_extend_kernel, dim3(1), dim3(KVP_THREADS), 0, ctx->stream, pages_of(pool), d_offsets, (int)rows, d_start, w,
+                             ctx->d_status));
     YSCV_CUDA_TRY(cudaGetLastError());
     ctx->launches++;
     KvApply a = apply_of(pool);
