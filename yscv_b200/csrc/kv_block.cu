@@ -138,7 +138,7 @@ __device__ __forceinline__ void kv_turn(const uint32_t (&w)[4], uint32_t (&out)[
 
 // (D: the head size, 0 for any; a division by it is a shift where it is known)
 template <int T, int D>
-__global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l, const float *__restrict__ k, const float *__restrict__ v, const KvRows rows,
+__global__ void __launch_bounds__(T, 1024 / T) kv_append_kernel(const KvLayer l, const float *k, const float *v, const KvRows rows,
                                                       int per_seq, int wide, int *__restrict__ status) {
     extern __shared__ __align__(16) unsigned char stage[];   // [tokens][kv_stage_pitch(d)]
     __shared__ float red[T / 32];

@@ -168,7 +168,7 @@ __device__ __forceinline__ KvGrowth growth_of(const KvPages &a, const int32_t *o
 
 constexpr int KVP_LISTED = 2048;   // free pages that are given out from shared memory
 
-__global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a, const int32_t *__restrict__ offsets, int rows,
+__global__ void __launch_bounds__(KVP_THREADS) kv_extend_kernel(const KvPages a, const int32_t *offsets, int rows,
                                                                 int32_t *__restrict__ start, const KvWork w, int *__restrict__ status) {
     __shared__ uint32_t sums[KVP_WARPS];
     __shared__ uint32_t seen[KVP_SEEN / 32];
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(KVP_THREADS) kv_compact_kernel(const KvPages a
 
 // ---- trim and fork: a warp per list entry ---------------------------------------------------------
 // The same sequence twice: an exchange gives a page to one of the two, the shorter length stays.
-__global__ void __launch_bounds__(256) kv_trim_kernel(const KvPages a, const int32_t *__restrict__ seqs, const int32_t *__restrict__ keep, int count,
+__global__ void __launch_bounds__(256) kv_trim_kernel(const KvPages a, const int32_t *seqs, const int32_t *keep, int count,
                                                       int *__restrict__ status) {
     pdl_wait();
     pdl_trigger();
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) kv_trim_kernel(const KvPages a, const int
 }
 
 // The lists are looked through for a second use of a number, so that what is left out does not depend on timing
-__global__ void __launch_bounds__(256) kv_fork_kernel(const KvPages a, const int32_t *__restrict__ src, const int32_t *__restrict__ dst, int count,
+__global__ void __launch_bounds__(256) kv_fork_kernel(const KvPages a, const int32_t *src, const int32_t *dst, int count,
                                                       int *__restrict__ status) {
     pdl_wait();
     pdl_trigger();
