@@ -762,7 +762,8 @@ int yscv_cuda_kv_block_read_rows_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
  * scale (scales down to 2^-80 of the largest among 128 keys; smaller ones count as that small). `rows` is the room in d_q and
  * d_out, at least d_offsets[n_seq]: a sequence whose offsets lie outside takes no part, status 4. Keys behind the table's
  * end are left out, status 3. Rows with a NaN or an infinity in the query are NaN, and only those. d_head 64, 128 or
- * 256. _workspace says how many bytes of device memory a call needs; calls that may overlap need one each. */
+ * 256. _workspace says how many bytes of device memory a call needs, and those with fewer rows or a smaller most_rows;
+ * calls that may overlap need one each. */
 int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows,
                                            size_t most_rows, size_t *bytes);
 int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_q,

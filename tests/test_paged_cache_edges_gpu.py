@@ -222,3 +222,27 @@ def test_pages_grow_without_positions():
     assert book.extend([2, 38, 1]) == (start.tolist(), 0)
     book.same(pool, before)
     ctx.close()
+
+
+@pytest.mark.parametrize("d,n_seq", [(64, 2), (128, 2), (256, 2), (64, 400), (128, 400)])
+@pytest.mark.parametrize("group", [1, 3, 8, 16, 40])
+def test_a_workspace_for_many_rows_serves_fewer(d, n_seq, group):
+    """A server has one workspace, sized for its longest prompt, for every call with as many heads: nothing behind it is written."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=60, n_kv=2, d=d, page=16, n_seq=n_seq, max_pages=30)
+    handle, rows = pool.handle(), 700
+    most = [0, 1, 2, 3, 5, 9, 17, 32, 33, 65, 600]
+    need = [ctx.kv_block_attention_workspace(handle, 2 * group, rows, m) for m in most]
+    assert need == sorted(need)
+    assert all(ctx.kv_block_attention_workspace(handle, 2 * group, r, most[-1]) <= need[-1] for r in (0, 1, 40, 699))
+    ws, guard = _guarded(need[-1])
+    pool.give([400] + [0] * (n_seq - 2) + [300])
+    q = torch.randn(40, 2 * group, d, device="cuda", generator=pool.g)
+    for m in (1, 2, 5, 20):
+        counts = [m] + [0] * (n_seq - 2) + [m // 2]
+        start = [400 - m] + [-1] * (n_seq - 2) + [290]
+        got, live = _attend(ctx, pool, q[:sum(counts)], counts, start, ws=ws[:need[-1]])
+        _done(ctx)
+        _check(got, live, *attention(pool, q[:sum(counts)], start, counts))
+        assert torch.equal(ws[need[-1]:], guard)
+    ctx.close()

@@ -654,9 +654,11 @@ template <int D, int R> static int ka_launch(yscv_cuda_ctx *ctx, const KvAttenti
     return YSCV_CUDA_OK;
 }
 
-static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t group, size_t rows, size_t most_rows) {
-    return kv_prompt_takes(pool, group, rows, most_rows) ? kv_prompt_bytes(ctx, pool->d_head)
-                                                                       : ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * group));
+// What any kernel needs that a call of so many rows, or of fewer, can run: who has sized a workspace for prompts decodes with it
+static size_t attention_bytes(const yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t group, size_t most_rows) {
+    size_t bytes = std::max(ka_bytes(ctx, pool->d_head, pool->n_seq, 8), ka_bytes(ctx, pool->d_head, pool->n_seq, ka_rows(pool->d_head, most_rows * group)));
+    if (kv_prompt_takes(pool, group, 0, most_rows)) bytes = std::max(bytes, kv_prompt_bytes(ctx, pool->d_head));
+    return bytes;
 }
 
 // A guess of no rows may be wrong: what a call launches and what it needs both go by one row at least
@@ -685,7 +687,7 @@ int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_k
                                            size_t *bytes) {
     if (const int rc = ka_check(ctx, pool, n_q, rows, most_rows)) return rc;
     if (!bytes) return fail(YSCV_CUDA_ERR_BAD_ARG, "bytes is null");
-    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, rows, ka_guess(most_rows));
+    *bytes = attention_bytes(ctx, pool, n_q / pool->n_kv, ka_guess(most_rows));
     return YSCV_CUDA_OK;
 }
 
@@ -705,7 +707,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     most_rows = ka_guess(most_rows);
     const size_t group = n_q / pool->n_kv, pairs = most_rows * group;
     const int R = ka_rows(pool->d_head, pairs);
-    const size_t need = attention_bytes(ctx, pool, group, rows, most_rows);
+    const size_t need = attention_bytes(ctx, pool, group, most_rows);
     if (workspace_bytes < need) return fail(YSCV_CUDA_ERR_BAD_ARG, "workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     if (rows == 0) return YSCV_CUDA_OK;
     YSCV_CUDA_TRY(cudaSetDevice(ctx->device));
