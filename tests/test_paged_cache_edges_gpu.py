@@ -246,3 +246,28 @@ def test_a_workspace_for_many_rows_serves_fewer(d, n_seq, group):
         _check(got, live, *attention(pool, q[:sum(counts)], start, counts))
         assert torch.equal(ws[need[-1]:], guard)
     ctx.close()
+
+
+@pytest.mark.parametrize("most", [1, 40])
+def test_a_window_of_two_to_the_thirty(most):
+    """A billion keys, which one page holds again and again; the first ones, in front of the window, would take all the weight."""
+    ctx = _context()
+    window = 1 << 30
+    start = window + 200
+    pool = Pool(ctx, n_pages=2, n_kv=1, d=64, page=128, n_seq=1, max_pages=(1 << 23) + 2)
+    q = torch.randn(1, 1, 64, device="cuda", generator=pool.g)
+    pool.table.fill_(1)
+    pool.table[0, 0] = 0                                # keys 0 .. 127: along the query
+    flat = (127.0 * torch.sign(q[0, 0])).to(torch.int8).expand(128, 64)
+    pool.k[0, 0, 0] = flat.reshape(8, 16, 4, 16).permute(0, 2, 1, 3)
+    pool.v[0, 0] = 127
+    pool.ks[0, 0], pool.ks[0, 1] = 0.05, 0.01
+    got, _ = _attend(ctx, pool, q, [1], [start], window=window, most=most)
+    assert ("tcgen05" in ctx.last_kernel()) == (most == 40)
+    _done(ctx)
+    k, v = pool.rows(0, 256)
+    p = torch.softmax(k[128:, 0] @ q[0, 0].double() / 8.0, 0)
+    # every key of the page 2^23 times, give or take one; sums over the steps of a warp, 2^24 / (148 * 12), or the tiles of an SM, 2^23 / 148
+    tol = (2.0 ** -22 + 2.0 ** -18 + 2.0 ** 16 * 2.0 ** -23) * float(v[128:].abs().max())
+    assert float((got[0, 0].double() - p @ v[128:, 0]).abs().max()) < tol
+    ctx.close()

@@ -720,7 +720,7 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
     a.n_q = (int)n_q;
     a.group = (int)group;
     a.causal = causal != 0;
-    a.window = (int)(window < (1u << 30) ? window : 0);
+    a.window = (int)(window < (1u << 31) ? window : 0);   // (no position is farther than that)
     a.wide = ((reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_out)) & 15) == 0 && q_stride % 4 == 0 && out_stride % 4 == 0;
     a.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)pool->d_head)) * 1.4426950408889634f;
     a.rows = (int)rows;
