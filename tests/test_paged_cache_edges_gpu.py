@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from paged_pool import Pool, attention, i32
-from test_paged_cache_gpu import Book, _append, _attend, _check, _context, _done, _expect_append, _refused, _same
+from test_paged_cache_gpu import Book, _append, _attend, _check, _context, _done, _expect_append, _extend, _positions, _refused, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -270,4 +270,33 @@ def test_a_window_of_two_to_the_thirty(most):
     # every key of the page 2^23 times, give or take one; sums over the steps of a warp, 2^24 / (148 * 12), or the tiles of an SM, 2^23 / 148
     tol = (2.0 ** -22 + 2.0 ** -18 + 2.0 ** 16 * 2.0 ** -23) * float(v[128:].abs().max())
     assert float((got[0, 0].double() - p @ v[128:, 0]).abs().max()) < tol
+    ctx.close()
+
+
+def test_pages_of_a_pool_that_shared_memory_has_no_bits_for():
+    """More than 131072 pages: those behind are looked up again, for the free ones and for what moves."""
+    ctx = _context()
+    pool = Pool(ctx, n_pages=150000, n_kv=1, d=16, page=16, n_seq=40, max_pages=3800)
+    tokens = [60000 - 7 * i for i in range(36)] + [0] * 4
+    pool.give(tokens)
+    book, handle = Book(pool), pool.handle()
+    ws = torch.empty(ctx.kv_pages_workspace(handle), dtype=torch.uint8, device="cuda").random_(0, 256)
+    new = [17] * 36 + [40000, 9, 0, 1]
+    for turn in range(2):
+        before = pool.state()
+        start, pos = _extend(ctx, pool, new)
+        want, status = book.extend(new)
+        assert status == 0 and start == want and pos == _positions(want, new)
+        _done(ctx)
+        book.same(pool, before)
+        gone = [1, 5, 36]
+        seqs = i32(gone)
+        before = pool.state()
+        torch.cuda.synchronize()
+        ctx.kv_pages_trim_dev(handle, seqs.data_ptr(), None, 3)
+        ctx.kv_pages_compact_dev(handle, ws.data_ptr(), ws.numel())
+        _done(ctx)
+        book.trim(gone, [0] * 3)
+        book.compact()
+        book.same(pool, before)
     ctx.close()
