@@ -85,6 +85,8 @@ def _by_what_a_row_sees(pool, q, start, counts, causal, window):
     n_q, d, n_kv = q.shape[1], q.shape[2], pool.n_kv
     out, tol, row = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda"), 0
     for i, (s0, m) in enumerate(zip(start, counts)):
+        if m == 0:
+            continue
         k, v = pool.rows(i, s0 + m)
         here, key = torch.arange(s0, s0 + m, device="cuda")[:, None], torch.arange(s0 + m, device="cuda")[None, :]
         hidden = (key > here) if causal else torch.zeros_like(key > here)
@@ -104,7 +106,7 @@ def _by_what_a_row_sees(pool, q, start, counts, causal, window):
     return out, tol
 
 
-@pytest.mark.parametrize("d,most", [(64, 2), (128, 2), (256, 2), (64, 80), (128, 80)])
+@pytest.mark.parametrize("d,most", [(64, 2), (128, 2), (256, 2), (64, 4), (128, 4), (64, 80), (128, 80)])
 @pytest.mark.parametrize("causal,window", [(True, 0), (True, 1), (True, 23), (False, 40)])
 @pytest.mark.parametrize("octaves", [12, 36, 70])
 def test_attention_over_pages_of_very_unlike_values(d, most, causal, window, octaves):
