@@ -682,7 +682,7 @@ int yscv_cuda_decoder_layers_dev(yscv_cuda_ctx *ctx, const yscv_cuda_decode_laye
  *   BANDED  by the turns of a pair over original_positions: at most low_band w_i / factor, at least
  *           high_band w_i, blended between
  *   YARN    the same with a ramp over the pairs, from the one that makes beta_fast turns over
- *           original_positions to the one that makes beta_slow
+ *           original_positions (rounded down) to the one that makes beta_slow (rounded up)
  * attention_factor multiplies cosine and sine (0: 0.1 ln(factor) + 1 with YARN, else 1). Angles are
  * formed in fp64. rotary_dim is even, at most d_head and 512. */
 enum {
@@ -758,12 +758,13 @@ int yscv_cuda_kv_block_read_rows_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
  * row without `causal`; with window > 0 only over keys after its own position minus window. scale 0
  * stands for 1 / sqrt(d_head). out rows are out_stride floats apart and may not overlap d_q; a row that sees no
  * key is 0. Cached numbers enter the products as they are, queries and softmax weights to 22 bits or more: as three
- * 8-bit digits and integer products for a few rows a sequence, as two fp16 terms for more; a weight together with its page's value
- * scale (scales down to 2^-80 of the largest among 128 keys; smaller ones count as that small). `rows` is the room in d_q and
- * d_out, at least d_offsets[n_seq]: a sequence whose offsets lie outside takes no part, status 4. Keys behind the table's
- * end are left out, status 3. Rows with a NaN or an infinity in the query are NaN, and only those. d_head 64, 128 or
- * 256. _workspace says how many bytes of device memory a call needs, and those with fewer rows or a smaller most_rows;
- * calls that may overlap need one each. */
+ * 8-bit digits and integer products for a few rows a sequence, as two fp16 terms for more; a weight together with
+ * its page's value scale (scales down to 2^-80 of the largest among 128 keys; smaller ones count as that small).
+ * `rows` is the room in d_q and d_out, at least d_offsets[n_seq]: a sequence whose offsets lie outside takes no part,
+ * status 4. Keys behind the table's end are left out, status 3. Rows with a NaN or an infinity in the query are NaN,
+ * and only those, as long as scores and sums of weights times values stay within fp32. d_head 64, 128 or 256, pools
+ * of up to 2160 sequences (heads of 64: 6250). _workspace says how many bytes of device memory a call needs, and
+ * those with fewer rows or a smaller most_rows; calls that may overlap need one each. */
 int yscv_cuda_kv_block_attention_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t n_q, size_t rows,
                                            size_t most_rows, size_t *bytes);
 int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t layer, const float *d_q,
@@ -786,8 +787,8 @@ int yscv_cuda_kv_block_attention_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool
  * fork: the empty sequence d_dst[j] shares all pages of d_src[j]. A source that is a destination of the same
  *   call, a destination that is not empty or appears a second time: left out, status 4.
  * compact: the used pages move to the lowest numbers, the k-th used one above into the k-th gap.
- * copy: page d_dst[j] becomes what d_src[j] is; negative numbers are passed over. No page may be both a
- *   source and a destination.
+ * copy: page d_dst[j] becomes what d_src[j] is; negative numbers are passed over. No page may be a
+ *   destination twice, or both a source and a destination (but of itself): what it holds then is not defined.
  * _workspace: bytes that extend and compact need. */
 int yscv_cuda_kv_pages_workspace(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, size_t *bytes);
 int yscv_cuda_kv_pages_extend_dev(yscv_cuda_ctx *ctx, const yscv_cuda_kv_pool *pool, const int32_t *d_offsets,

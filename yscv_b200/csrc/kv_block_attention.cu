@@ -19,8 +19,8 @@
 //
 // A step is a chain of some 1100 instructions, so what counts is how many warps an SM has, and their buffers: with two stages of both
 // operands and six warps at D = 128 the chain's latencies showed (64 sequences of 1000 to 8000 keys, 64 / 8 heads of 128: 133 us, IPC
-// 0.3 per scheduler); one place each for keys and values gives twelve: 112 us. With both products taken out the kernel takes 106: what
-// bounds it is the fetching of 8 KB pieces from all over the pool, 5.6 TB/s with its beginning and end.
+// 0.3 per scheduler); one place each for keys and values gives twelve: 114 us, 118 with the joining kernel. With both products taken out
+// the kernel took 106: what bounds it is the fetching of 8 KB pieces from all over the pool, 5.6 TB/s with its beginning and end.
 //
 // R = 8: the 16 rows of a product hold two digits of eight pairs, two products per tile instead of three.
 // Bound: the cache's bytes from HBM (594 MB there, 92 us at the copy rate).

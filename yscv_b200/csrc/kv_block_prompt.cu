@@ -23,8 +23,8 @@
 // Work: the tiles of all (sequence, pairs, KV head) segments are laid end to end, KP_TILE places each, with KP_BEGIN places in front of
 // each segment, about what its beginning and end take, and every SM takes an equal run; a segment that several SMs share leaves records, which
 // kv_prompt_merge_kernel adds. So a short piece over a long cache fills the machine too, and causal prompts, whose first
-// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128: 151 us where it took 162 with four
-// places in front of a segment, 154 with five; 146 now).
+// segments have one tile, need no order of CTAs (2047 tokens, 64 / 8 heads of 128, in runs of a few calls: 151 us where it took 162
+// with four places in front of a segment, 154 with five. A call among many takes 164, at a lower clock).
 // Bound: the tensor pipe, 2 x (128 D + 128 D) x 128 MACs a tile, 2048 cycles at the nominal rate for D = 128; what holds a tile for 3600
 // is the chain of its two products and its softmax, with as many tiles on their way as TMEM has room for (two), and the issue slots,
 // of which a tile takes 2100 of each scheduler.
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) kv_prompt_kernel(const __grid_c
                 for (int j = 0; j < D / 2; ++j) o[j] = 0ull;
             }
             // What the output is relative to follows the maximum only where that is 2^8 above it, which after a segment's first tiles is
-            // rare (pieces of three prompts: 88 us, 91 with a factor on the output for every tile)
+            // rare (pieces of three prompts, in runs of a few calls: 88 us, 91 with a factor on the output for every tile)
             if (__any_sync(0xffffffffu, ms.x > m + 8.0f)) {
                 const float m_new = fmaxf(m, ms.x), alpha = m_new == -INFINITY ? 1.0f : at_exp2(m - m_new);
                 const uint64_t al2 = f2(alpha, alpha);
